@@ -336,6 +336,69 @@ IFLB200_API int iflb200_quant_from_amax(const float* h, int64_t ld_h, int M, int
                             void* q, int64_t ld_q, float* qs, void* stream);
 
 /*
+ * Quantiser with a scale for each row and block of 128 columns:
+ *   amax = max(max |v| over the block, 1e-8);  qs[m, b] = amax / 448;  q[m, k] = e4m3(v * (448 / amax))
+ * with IEEE divisions.  act -1: v = x, x [M, K]; IFLB200_ACT_*: v = act(x[m, k]) * x[m, K + k], x [M, 2K].
+ * qs[m * qs_row + b * qs_block].  Any K, any strides.  An infinity or NaN makes its block's scale infinite or NaN.
+ * No reference counterpart (its quantisers have one scale a row).
+ */
+IFLB200_API int iflb200_block_quant(const void* x, int x_dtype, int64_t ld_x, int M, int K, int act, void* q, int64_t ld_q,
+                                    float* qs, int64_t qs_row, int64_t qs_block, void* stream);
+
+/*
+ * GEMM of operands with block scales:
+ *   out[m, n] = out_dtype(sum_b a_scale[m, b] w_scale[n / 128, b] sum_{k in block b} a[m, k] w[n, k]  (+ bias[n]))
+ * a_scale[m * a_scale_row + b * a_scale_block]; w_scale dense [ceil(N / 128)][ceil(K / 128)]; bias float32 or bf16.
+ * All sums in fp32, one rounding.  K and N multiples of 16, rows of a, w and out 16-byte aligned.  Stream ordering of w as
+ * for iflb200_gemm_fp8_raw.  Few output tiles share the K range among the CTAs of a cluster; partial sums are added in
+ * the order of the ranges, so the result does not depend on timing.
+ * No reference counterpart.
+ */
+IFLB200_API int iflb200_block_linear(const void* a, int64_t ld_a, const void* w, int64_t ld_w, int M, int N, int K,
+                                     const float* a_scale, int64_t a_scale_row, int64_t a_scale_block, const float* w_scale,
+                                     const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ld_out, void* stream);
+
+/*
+ * Tuning: form of iflb200_block_linear (0 by rule, 1 single CTAs, 2 CTA pairs, 3 pairs with two K steps a stage), tokens
+ * of a tile (0 by rule; a multiple of 16 up to 256, up to 128 for forms 1 and 3) and, for form 1, the CTAs that share a
+ * tile's K range (0 by rule, up to 8).
+ */
+IFLB200_API int iflb200_block_linear_set_form(int form, int tokens, int splits);
+
+/*
+ * New keys and values into an 8-bit paged cache: k and v [B, T, heads, head_dim] (strides in elements, last dimension
+ * contiguous) to the codes [pages][heads][page_tokens][head_dim] and scales [pages][heads], at positions start[b] + t of
+ * the sequence whose pages are table[b * ld_table + 0 .. max_pages).  A page's scale is the least power of two that brings
+ * its largest finite value to 448 or below and never falls; codes below start[b] are rescaled where it grows.  counts
+ * (optional): tokens of each row that are there.  Tokens whose page is beyond the table or outside 0 .. pages - 1 are
+ * dropped.  head_dim 64, 128 or 256; page_tokens a multiple of 16 up to 256.
+ * No reference counterpart.
+ */
+IFLB200_API int iflb200_cache_append(const void* k, int64_t k_b, int64_t k_t, int64_t k_h, const void* v, int64_t v_b, int64_t v_t,
+                                     int64_t v_h, int dtype, int B, int T, int heads, int head_dim, void* k_codes, void* v_codes,
+                                     float* k_scale, float* v_scale, int pages, int page_tokens, const int32_t* table,
+                                     int64_t ld_table, int max_pages, const int32_t* start, const int32_t* counts, void* stream);
+
+/*
+ * Attention over that cache: q and out [B, T, heads_q, head_dim] (bf16 or f16, strides in elements, last dimension
+ * contiguous), query head i reads head i / (heads_q / heads_kv).  Token t of the q_lens[b] (T without it) of row b stands at
+ * p = lens[b] - q_lens[b] + t.
+ *   s_j = scale * q.k_j;  softcap > 0: s_j = softcap * tanh(s_j / softcap);  slopes: s_j -= slopes[i] * |p - j|
+ *   out = sum_j softmax(s)_j v_j  over the keys j < lens[b] and, with causal, j <= p or j < prefix[b] (prefix optional)
+ * Scores, weights' sum and output are accumulated in fp32, the weights enter the product as f16.  Rows that see no key are
+ * zeros; rows t >= q_lens[b] are not written.  workspace (optional, 16-byte aligned): scratch that lets several CTAs
+ * share a sequence; its first 4096 bytes have to be zero and are left so.  Calls that may overlap need one each.
+ * No reference counterpart (its cache is 16-bit).
+ */
+IFLB200_API int iflb200_cache_attention(const void* q, int dtype, int64_t q_b, int64_t q_t, int64_t q_h, const void* k_codes,
+                                        const void* v_codes, const float* k_scale, const float* v_scale, int pages,
+                                        int page_tokens, int head_dim, const int32_t* table, int64_t ld_table, int max_pages,
+                                        const int32_t* lens, const int32_t* q_lens, const int32_t* prefix, const float* slopes,
+                                        int B, int T, int heads_q, int heads_kv, float scale, float softcap, int causal,
+                                        void* out, int64_t o_b, int64_t o_t, int64_t o_h, void* workspace,
+                                        int64_t workspace_bytes, void* stream);
+
+/*
  * Per-tensor dynamic e4m3 pack (the torch-FP8-linear recipe):
  *   amax = max |x| (NaN propagates);  scale = max(amax, 1e-12) * fp32(1/448);
  *   q = e4m3_rn(clamp(x / scale, -448, 448))   (IEEE division, NaN propagates)

@@ -25,6 +25,9 @@ SOURCES = (("gemm_fp8_sm100.cu", (), "gemm_fp8_sm100"),
            ("attn_ops.cu", (), "attn_ops"),
            ("xgpu_ops.cu", (), "xgpu_ops"),
            ("row_stream.cu", (), "row_stream"),
+           ("block_ops.cu", (), "block_ops"),
+           ("gemm_block.cu", (), "gemm_block"),
+           ("cache_attn.cu", (), "cache_attn"),
            ("row_ops.cu", ("-DIFLB200_ROW_PART=0",), "row_ops_quant"),
            ("row_ops.cu", ("-DIFLB200_ROW_PART=1",), "row_ops_gated_pack"),
            ("row_ops.cu", ("-DIFLB200_ROW_PART=2",), "row_ops_resnorm"))

@@ -1,0 +1,689 @@
+// FP8 GEMM whose operands have a scale for each block of 128: activations for each row and 128 columns, weights for
+// each 128 x 128 block.
+//
+//   out[t, n] = out_type( sum_b sa[t, b] sw[n / 128, b] * ( sum_{k in block b} A[t, k] W[n, k] )  (+ bias[n]) )
+//
+// The inner sums run on tcgen05 (fp32 accumulators in tensor memory).  A scale changes from one K step of 128 to the
+// next, so the accumulator of every step is taken out of tensor memory, multiplied and added to a sum in the epilogue
+// warps' registers (fp32 throughout), while the MMAs of the next step run into another accumulator.
+//
+// Weights are on the MMA's M side (128 rows a CTA: one row of weight blocks, so one weight scale a step), tokens on its
+// N side in tiles of any multiple of 16: the accumulator is the tile transposed.  Sixteen warps take it out in the
+// 16 x 256-bit shape, where a thread holds four weight rows of two neighbouring tokens: one 8-byte read of the tokens'
+// scales serves four packed fused multiply-adds.
+//
+//   warp 0      TMA producer of W         warp 1   MMA issuer, tensor memory
+//   warp 2      TMA producer of A         warp 3   scales: sa * sw of the step into shared memory
+//   warps 4..19 promotion and epilogue
+//
+// CG 2 works on CTA pairs (256 weight rows), CG 1 on single CTAs, whose K range a cluster of up to eight may share:
+// the partial sums meet in distributed shared memory and are added in the order of the ranges.  SL: K steps of a
+// stage; two of them share one commit where tiles are narrow (a commit occupies the issuing thread for 320 clocks).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "../../include/iflb200.h"
+#include "launch.cuh"
+#include "rowmath.cuh"
+
+namespace iflb200 {
+
+namespace {
+
+constexpr int kStep = 128;  // bytes of K and weight rows: a block of the weight
+constexpr int kEpi = 16;    // epilogue warps
+constexpr int kThreads = 32 * (4 + kEpi);
+constexpr uint64_t kBudgetNs = 2000000000ull;
+constexpr int kMaxStages = 8;
+constexpr int kMaxSmem = 227 * 1024;
+
+__device__ uint32_t g_record[4];
+__device__ uint64_t g_budget_ns = kBudgetNs;
+
+struct BlockParams {
+  int M, N, K;
+  int bt;                                // tokens of a tile
+  int num_m, num_n, num_k, units, group_m;
+  int splits;                            // CG 1: CTAs of a cluster that share a tile's K range
+  int stages;
+  uint32_t idesc;
+  const float* sa;
+  int64_t sa_row, sa_block;
+  const float* sw;                       // [ceil(N / 128)][num_k]
+  const void* bias;
+  int bias_dtype;
+  uint8_t* out;
+  int64_t ld_out;                        // bytes
+  int out_dtype;
+  int staging;                           // bytes a warp: 16 tokens x 32 columns
+  int early;                             // the first weights may be read ahead of the dependency wait
+};
+
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void store_transposed(uint32_t addr, const uint32_t (&v)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint64_t lds64(uint32_t addr) {
+  uint64_t v;
+  asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts32(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster_64x2(uint32_t addr, uint32_t rank, uint64_t a, uint64_t b) {
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
+      "st.shared::cluster.v2.b64 [ra], {%2, %3};\n\t}"
+      ::"r"(addr), "r"(rank), "l"(a), "l"(b)
+      : "memory");
+}
+
+// Bounded wait of one thread; false once the CTA gives up.
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = 0;
+  uint32_t spins = 0;
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (++spins > 2048) {
+      if (t0 == 0) t0 = globaltimer_ns();
+      __nanosleep(128);
+      if (globaltimer_ns() - t0 > g_budget_ns) {
+        *abort = 1;
+        atomicCAS(&g_record[0], 0u, code);
+        return false;
+      }
+    }
+  }
+}
+// The same for a converged warp.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t code) {
+  if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
+  const bool ok = wait_one(bar, parity, abort, code);
+  return __all_sync(0xFFFFFFFFu, ok);
+}
+
+__device__ __forceinline__ uint32_t pair_bf16(float a, float b) {
+  return f32_to_bf16_bits(a) | (f32_to_bf16_bits(b) << 16);
+}
+__device__ __forceinline__ uint32_t pair_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int CG, int SL>
+struct Layout {
+  static constexpr int kAcc = 256 / SL;                     // tensor-memory columns of an accumulator: two stages of SL
+  static constexpr int kScales = 2 * SL * kAcc * 4;         // bytes
+  __host__ __device__ static int slab(int bt) { return kStep * kStep + bt / CG * kStep; }
+  static int blocks_of(int bt, int splits) { return (bt / 16 + splits - 1) / splits; }  // token blocks that a rank adds up
+  static int meeting(int bt, int splits) { return splits > 1 ? blocks_of(bt, splits) * splits * 4 * 2048 : 0; }
+  static int fixed(int bt, int splits, int staging) {
+    return 1024 + kEpi * staging + kScales + meeting(bt, splits) + (2 * kMaxStages + 8) * 8 + 16;
+  }
+  static int stages(int bt, int splits, int staging) {
+    const int n = (kMaxSmem - fixed(bt, splits, staging)) / (SL * slab(bt));
+    return n < kMaxStages ? n : kMaxStages;
+  }
+};
+
+template <int CG, int SL>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_constant__ CUtensorMap tm_w,
+                      const __grid_constant__ BlockParams p) {
+  using L = Layout<CG, SL>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw_addr);
+  const int stages = p.stages;
+  const uint32_t w_bytes = kStep * kStep, t_bytes = (uint32_t)(p.bt / CG) * kStep, slab_bytes = w_bytes + t_bytes;
+  const uint32_t staging0 = base + stages * SL * slab_bytes;
+  const uint32_t scales0 = staging0 + kEpi * p.staging;
+  const uint32_t meeting0 = scales0 + L::kScales;
+  const int own_blocks = CG == 1 && p.splits > 1 ? (p.bt / 16 + p.splits - 1) / p.splits : 0;
+  const uint32_t bar0 = meeting0 + (uint32_t)(own_blocks * p.splits) * 4 * 2048;
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto done_bar = [&](int s) { return bar0 + 8u * (kMaxStages + s); };      // MMAs of the stage complete: slabs free, accumulators full
+  auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kMaxStages + a); };
+  auto sfull_bar = [&](int a) { return bar0 + 8u * (2 * kMaxStages + 2 + a); };
+  auto sempty_bar = [&](int a) { return bar0 + 8u * (2 * kMaxStages + 4 + a); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar0 - base) + (2 * kMaxStages + 8) * 8);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = CG == 1 || rank == 0;
+  const int splits = CG == 1 ? p.splits : 1;
+  const int width = CG == 1 ? splits : 2;
+  const int first_unit = blockIdx.x / width, unit_stride = gridDim.x / width;
+  // this CTA's K range, in blocks
+  const int kb0 = CG == 1 ? (int)((int64_t)p.num_k * rank / splits) : 0;
+  const int kb1 = CG == 1 ? (int)((int64_t)p.num_k * (rank + 1) / splits) : p.num_k;
+  auto place = [&](int unit, int& t_blk, int& w_blk) {
+    const int band = p.group_m * p.num_n, g = unit / band;
+    const int first = g * p.group_m, size = min(p.num_m - first, p.group_m), r = unit - g * band;
+    t_blk = first + r % size;
+    w_blk = r / size;
+  };
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_t);
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(full_bar(i), 2);
+      mbar_init(done_bar(i), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tempty_bar(a), CG * kEpi);
+      mbar_init(sfull_bar(a), 1);
+      mbar_init(sempty_bar(a), kEpi);
+    }
+    tmem_slot[1] = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  __syncwarp();
+  cluster_arrive();
+  if (warp == 1) {
+    if (CG == 2) {
+      tmem_alloc_pair(smem_u32(tmem_slot), 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), 512);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  cluster_wait();
+
+  uint64_t acc[4][8];  // sums of the epilogue warps: token block, then half * 4 + group of 8 tokens * 2 + row of 8
+  const int quad = warp & 3, part = (warp - 4) >> 2;
+  const int r4 = lane >> 2, c4 = lane & 3;
+
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------------------ TMA producers
+    const bool weights = warp == 0;
+    if (elect_one()) {
+      bool waited = weights && p.early, ok = true;
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int unit = first_unit; ok && unit < p.units; unit += unit_stride) {
+        int t_blk, w_blk;
+        place(unit, t_blk, w_blk);
+        const int w_row = (w_blk * CG + (CG == 2 ? (int)rank : 0)) * kStep;
+        const int t_row = t_blk * p.bt + (CG == 2 ? (int)rank * (p.bt / 2) : 0);
+        for (int kb = kb0; kb < kb1; kb += SL) {
+          ok = wait_one(done_bar(stage), phase ^ 1, abort_flag, (1u << 24) | (1u << 16) | (uint32_t)(kb & 0xFFFF));
+          if (!ok) break;
+          const int slabs = min(SL, kb1 - kb);
+          const uint32_t bar = full_bar(stage), dst = base + stage * SL * slab_bytes + (weights ? 0u : w_bytes);
+          if (leader) mbar_arrive_expect_tx(bar, (uint32_t)(CG * slabs) * (weights ? w_bytes : t_bytes));
+          if (!waited) grid_dependency_wait();
+          waited = true;
+          for (int h = 0; h < slabs; ++h) {
+            const int x = (kb + h) * kStep;
+            if (CG == 2) {
+              tma_load_2d_pair(dst + h * slab_bytes, weights ? &tm_w : &tm_t, bar & kPeerBitMask, x, weights ? w_row : t_row);
+            } else {
+              tma_load_2d(dst + h * slab_bytes, weights ? &tm_w : &tm_t, bar, x, weights ? w_row : t_row);
+            }
+          }
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!weights) {
+        grid_dependency_wait();
+        grid_launch_dependents();
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (leader && elect_one()) {
+      bool ok = true;
+      int stage = 0;
+      uint32_t phase = 0, it = 0;
+      const uint64_t dw0 = make_kmajor_sw128_desc(base), dt0 = make_kmajor_sw128_desc(base + w_bytes);
+      for (int unit = first_unit; ok && unit < p.units; unit += unit_stride) {
+        for (int kb = kb0; kb < kb1; kb += SL, ++it) {
+          const uint32_t a = it & 1u;
+          ok = wait_one(tempty_bar(a), ((it >> 1) & 1u) ^ 1u, abort_flag, (2u << 24) | (2u << 16) | (it & 0xFFFF)) &&
+               wait_one(full_bar(stage), phase, abort_flag, (2u << 24) | (3u << 16) | (it & 0xFFFF));
+          if (!ok) break;
+          tc_fence_after();
+          const int slabs = min(SL, kb1 - kb);
+          for (int h = 0; h < slabs; ++h) {
+            const uint64_t at = (uint64_t)(((stage * SL + h) * slab_bytes) >> 4);
+            const uint32_t d = tmem_base + (a * SL + h) * L::kAcc;
+#pragma unroll
+            for (int j = 0; j < kStep / 32; ++j) {
+              if (CG == 2) mma_f8f6f4_pair(d, dw0 + at + 2 * j, dt0 + at + 2 * j, p.idesc, j > 0);
+              else mma_f8f6f4(d, dw0 + at + 2 * j, dt0 + at + 2 * j, p.idesc, j > 0);
+            }
+          }
+          if (CG == 2) mma_commit_pair(done_bar(stage), 3);
+          else mma_commit(done_bar(stage));
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ scales
+    // Read in batches of several steps, 32 values a lane in flight: one trip to L2 a batch.
+    constexpr int TPL = L::kAcc / 32, BATCH = 32 / TPL;
+    bool ok = true;
+    uint32_t it = 0;
+    grid_dependency_wait();
+    for (int unit = first_unit; ok && unit < p.units; unit += unit_stride) {
+      int t_blk, w_blk;
+      place(unit, t_blk, w_blk);
+      const int nb = min(w_blk * CG + (CG == 2 ? (int)rank : 0), (p.N - 1) / kStep);
+      const float* sw = p.sw + (int64_t)nb * p.num_k;
+      const float* sa[TPL];
+#pragma unroll
+      for (int i = 0; i < TPL; ++i) sa[i] = p.sa + (int64_t)min(t_blk * p.bt + 32 * i + lane, p.M - 1) * p.sa_row;
+      for (int kb = kb0; ok && kb < kb1; kb += BATCH) {
+        float v[BATCH][TPL], w[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          w[j] = kb + j < kb1 ? __ldg(sw + kb + j) : 0.0f;
+#pragma unroll
+          for (int i = 0; i < TPL; ++i)
+            v[j][i] = kb + j < kb1 && 32 * i + lane < p.bt ? __ldg(sa[i] + (int64_t)(kb + j) * p.sa_block) : 0.0f;
+        }
+#pragma unroll
+        for (int s = 0; s < BATCH / SL; ++s) {
+          if (ok && kb + s * SL < kb1) {
+            const uint32_t a = it & 1u;
+            ok = wait_warp(sempty_bar(a), ((it >> 1) & 1u) ^ 1u, abort_flag, (4u << 24) | (5u << 16) | (it & 0xFFFF));
+            if (ok) {
+#pragma unroll
+              for (int h = 0; h < SL; ++h) {
+#pragma unroll
+                for (int i = 0; i < TPL; ++i)
+                  sts32(scales0 + ((a * SL + h) * L::kAcc + 32 * i + lane) * 4, v[s * SL + h][i] * w[s * SL + h]);
+              }
+              __syncwarp();
+              if (lane == 0) mbar_arrive(sfull_bar(a));
+              ++it;
+            }
+          }
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ promotion, epilogue
+    bool ok = true;
+    int stage = 0;
+    uint32_t phase = 0, it = 0;
+    const uint32_t staging = staging0 + (uint32_t)(warp - 4) * p.staging;
+    // bias and stores of one block of 16 tokens
+    auto store = [&](const uint64_t (&s)[8], int tok, int n0, const float (&bs)[4]) {
+      __syncwarp();  // the block before this one has left the staging buffer
+      if (p.out_dtype == IFLB200_F32) {
+        // 128-byte rows of 32 columns, 16-byte pieces swizzled by the token
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int half = i >> 2, j = (i >> 1) & 1, sub = i & 1;
+          float v[2];
+          unpack2(s[i], v[0], v[1]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t chunk = (uint32_t)(4 * half + 2 * sub + (lane >> 4)) ^ (uint32_t)(2 * c4 + e);
+            sts32(staging + (8 * j + 2 * c4 + e) * 128 + chunk * 16 + (r4 & 3) * 4, v[e] + bs[2 * half + sub]);
+          }
+        }
+        __syncwarp();
+        uint8_t* o = p.out + (int64_t)(tok + (lane >> 3)) * p.ld_out + (int64_t)n0 * 4 + (lane & 7) * 16;
+        const bool in = n0 + 4 * (lane & 7) < p.N;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = 4 * i + (lane >> 3);
+          const uint4 v = lds128(staging + t * 128 + (((lane & 7) ^ (t & 7)) << 4));
+          if (in && tok + t < p.M) *reinterpret_cast<uint4*>(o + 4 * i * p.ld_out) = v;
+        }
+      } else {
+        // 64-byte rows of 32 columns, pieces swizzled by the token pair: four 8 x 8 matrices a store, transposed on the way
+        const uint32_t row = (uint32_t)(lane & 7), chunk = (uint32_t)(lane >> 3) ^ (row >> 1 & 3);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float a, b;
+            unpack2(s[(i >> 1) * 4 + j * 2 + (i & 1)], a, b);
+            a += bs[i];
+            b += bs[i];
+            v[i] = p.out_dtype == IFLB200_F16 ? pair_f16(a, b) : pair_bf16(a, b);
+          }
+          store_transposed(staging + (8 * j + row) * 64 + chunk * 16, v);
+        }
+        __syncwarp();
+        uint8_t* o = p.out + (int64_t)(tok + r4) * p.ld_out + (int64_t)n0 * 2 + c4 * 16;
+        const bool in = n0 + c4 * 8 < p.N;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 v = lds128(staging + (8 * i + r4) * 64 + ((c4 ^ (r4 >> 1 & 3)) << 4));
+          if (in && tok + 8 * i + r4 < p.M) *reinterpret_cast<uint4*>(o + 8 * i * p.ld_out) = v;
+        }
+      }
+    };
+    grid_dependency_wait();
+    for (int unit = first_unit; ok && unit < p.units; unit += unit_stride) {
+      int t_blk, w_blk;
+      place(unit, t_blk, w_blk);
+      const int tok_base = t_blk * p.bt;
+      const int n0 = (w_blk * CG + (CG == 2 ? (int)rank : 0)) * kStep + quad * 32;
+      const int blocks = n0 < p.N ? min(p.bt, p.M - tok_base + 15) / 16 : 0;
+      float bs[4] = {-0.0f, -0.0f, -0.0f, -0.0f};  // an addend of -0 changes nothing
+      if (p.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = n0 + 8 * i + r4;
+          if (n < p.N)
+            bs[i] = p.bias_dtype == IFLB200_F32 ? __ldg(reinterpret_cast<const float*>(p.bias) + n)
+                                                : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[n]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[b][i] = 0;
+      for (int kb = kb0; kb < kb1; kb += SL, ++it) {
+        const uint32_t a = it & 1u;
+        ok = wait_warp(sfull_bar(a), (it >> 1) & 1u, abort_flag, (3u << 24) | (6u << 16) | (it & 0xFFFF)) &&
+             wait_warp(done_bar(stage), phase, abort_flag, (3u << 24) | (4u << 16) | (it & 0xFFFF));
+        if (!ok) break;
+        tc_fence_after();
+        const int slabs = min(SL, kb1 - kb);
+#pragma unroll
+        for (int h = 0; h < SL; ++h) {
+          if (h < slabs) {
+            const uint32_t t_acc = tmem_base + ((uint32_t)(quad * 32) << 16) + (a * SL + h) * L::kAcc;
+            const uint32_t s_at = scales0 + ((a * SL + h) * L::kAcc + 2 * c4) * 4;
+#pragma unroll
+            for (int b = 0; b < (SL == 1 ? 4 : 2); ++b) {
+              const int block = part + 4 * b;
+              if (block < blocks) {
+                uint32_t r[16];
+                tmem_ld_16(t_acc + 16 * block, r);
+                tmem_ld_16(t_acc + (16u << 16) + 16 * block, r + 8);
+                const uint64_t s0 = lds64(s_at + 64 * block), s1 = lds64(s_at + 64 * block + 32);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  acc[b][i] = fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), (i >> 1) & 1 ? s1 : s0, acc[b][i]);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) mbar_arrive_cluster(tempty_bar(a), 0);
+          else mbar_arrive(tempty_bar(a));
+          mbar_arrive(sempty_bar(a));
+        }
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      if (CG == 1 && splits > 1) {
+        // to the rank that adds the block up: [own block][source rank][quadrant][piece][lane]
+#pragma unroll
+        for (int b = 0; b < (SL == 1 ? 4 : 2); ++b) {
+          const int block = part + 4 * b;
+          if (block < blocks) {
+            const uint32_t at = meeting0 + (uint32_t)(((block / splits) * splits + (int)rank) * 4 + quad) * 2048 + lane * 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st_cluster_64x2(at + i * 512, (uint32_t)(block % splits), acc[b][2 * i], acc[b][2 * i + 1]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < (SL == 1 ? 4 : 2); ++b) {
+          const int block = part + 4 * b;
+          if (block < blocks) store(acc[b], tok_base + 16 * block, n0, bs);
+        }
+      }
+    }
+    if (CG == 1 && splits > 1) {
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+      int t_blk, w_blk;
+      place(first_unit, t_blk, w_blk);
+      const int tok_base = t_blk * p.bt, n0 = w_blk * kStep + quad * 32;
+      const int blocks = n0 < p.N ? min(p.bt, p.M - tok_base + 15) / 16 : 0;
+      float bs[4] = {-0.0f, -0.0f, -0.0f, -0.0f};
+      if (p.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = n0 + 8 * i + r4;
+          if (n < p.N)
+            bs[i] = p.bias_dtype == IFLB200_F32 ? __ldg(reinterpret_cast<const float*>(p.bias) + n)
+                                                : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[n]);
+        }
+      }
+      for (int own = part; own < own_blocks; own += 4) {
+        const int block = own * splits + (int)rank;
+        if (ok && block < blocks) {
+          uint64_t s[8] = {};
+          for (int src = 0; src < splits; ++src) {
+            const uint32_t at = meeting0 + (uint32_t)((own * splits + src) * 4 + quad) * 2048 + lane * 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4 v = lds128(at + i * 512);
+              s[2 * i] = add2(s[2 * i], (uint64_t)v.x | ((uint64_t)v.y << 32));
+              s[2 * i + 1] = add2(s[2 * i + 1], (uint64_t)v.z | ((uint64_t)v.w << 32));
+            }
+          }
+          store(s, tok_base + 16 * block, n0, bs);
+        }
+      }
+    }
+  }
+  if (CG == 1 && splits > 1 && warp < 4) {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
+
+  // Neither CTA of a pair leaves while the other's MMAs, commits or arrivals can still reach it.
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);
+  }
+  tc_fence_before();
+  if (CG == 2) {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    if (CG == 2) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// --------------------------------------------------------------------------------------------
+// Host side
+// --------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                  CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(p);
+  }();
+  return fn;
+}
+
+// [rows, K] e4m3, box 128 bytes x box_rows with the 128-byte swizzle, zeros outside.
+int operand_map(CUtensorMap* tm, const void* ptr, int rows, int K, int64_t ld, int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return IFLB200_ERR_DRIVER;
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {(cuuint32_t)kStep, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? IFLB200_OK
+             : IFLB200_ERR_DRIVER;
+}
+
+// iflb200_block_linear_set_form; zeros: by rule
+int g_form = 0, g_tokens = 0, g_splits = 0;
+
+template <int CG, int SL>
+int launch_form(const void* a, int64_t ld_a, const void* w, int64_t ld_w, BlockParams p, int bt, int splits, int sms, cudaStream_t s) {
+  using L = Layout<CG, SL>;
+  static bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return IFLB200_ERR_DEVICE;
+  if (!attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_block_kernel<CG, SL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    if (e != cudaSuccess) return (int)e;
+    attr_set[dev] = true;
+  }
+  p.bt = bt;
+  p.splits = splits;
+  p.num_m = (p.M + bt - 1) / bt;
+  p.num_n = (p.N + CG * kStep - 1) / (CG * kStep);
+  p.num_k = (p.K + kStep - 1) / kStep;
+  p.units = p.num_m * p.num_n;
+  p.group_m = p.num_m <= 24 ? p.num_m : 16;
+  p.staging = p.out_dtype == IFLB200_F32 ? 2048 : 1024;
+  p.stages = L::stages(bt, splits, p.staging);
+  p.idesc = make_idesc_e4m3_f32(CG * kStep, bt);
+  CUtensorMap tt, tw;
+  int st = operand_map(&tt, a, p.M, p.K, ld_a, bt / CG);
+  if (st == IFLB200_OK) st = operand_map(&tw, w, p.N, p.K, ld_w, kStep);
+  if (st != IFLB200_OK) return st;
+  const int most = CG == 2 ? sms / 2 : sms;
+  const unsigned ctas = CG == 1 && splits > 1 ? (unsigned)(p.units * splits) : (unsigned)(CG * (p.units < most ? p.units : most));
+  const size_t smem = (size_t)L::fixed(bt, splits, p.staging) + (size_t)p.stages * SL * L::slab(bt);
+  const cudaError_t e = launch_dep(gemm_fp8_block_kernel<CG, SL>, dim3(ctas), dim3(kThreads), smem, s, CG == 2 ? 2 : splits,
+                                   dependent_launch_for(p.M, true), tt, tw, p);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+}  // namespace
+
+int set_block_wait_budget_ns(uint64_t ns) { return (int)cudaMemcpyToSymbol(g_budget_ns, &ns, sizeof(ns)); }
+
+// The record of a timed-out wait of this kernel, and clears it.
+int take_block_timeout_record(uint32_t* record, cudaStream_t s) {
+  uint32_t host[4] = {0, 0, 0, 0};
+  cudaError_t e = cudaMemcpyFromSymbolAsync(host, g_record, sizeof(host), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) return (int)e;
+  *record = host[0];
+  if (host[0] != 0) {
+    const uint32_t zero[4] = {0, 0, 0, 0};
+    e = cudaMemcpyToSymbolAsync(g_record, zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
+  return (int)e;
+}
+
+}  // namespace iflb200
+
+using namespace iflb200;
+
+extern "C" int iflb200_block_linear_set_form(int form, int tokens, int splits) {
+  if (form < 0 || form > 3 || tokens < 0 || tokens > 256 || tokens % 16 || splits < 0 || splits > 8) return IFLB200_ERR_ARG;
+  if (form != 2 && tokens > 128) return IFLB200_ERR_ARG;  // forms of two K steps a stage
+  if (form != 1 && splits > 1) return IFLB200_ERR_ARG;
+  g_form = form;
+  g_tokens = tokens;
+  g_splits = splits;
+  return IFLB200_OK;
+}
+
+extern "C" int iflb200_block_linear(const void* a, int64_t ld_a, const void* w, int64_t ld_w, int M, int N, int K,
+                                    const float* a_scale, int64_t a_scale_row, int64_t a_scale_block, const float* w_scale,
+                                    const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ld_out, void* stream) {
+  if (M < 0 || N < 0 || K < 0) return IFLB200_ERR_ARG;
+  if (out_dtype != IFLB200_F32 && out_dtype != IFLB200_BF16 && out_dtype != IFLB200_F16) return IFLB200_ERR_DTYPE;
+  if (bias && bias_dtype != IFLB200_F32 && bias_dtype != IFLB200_BF16) return IFLB200_ERR_DTYPE;
+  if (K % 16 || N % 16) return IFLB200_ERR_SHAPE;
+  if (M == 0 || N == 0) return IFLB200_OK;
+  if (K < 16) return IFLB200_ERR_SHAPE;
+  if (!a || !w || !out || !a_scale || !w_scale) return IFLB200_ERR_ARG;
+  if (ld_a < K || ld_w < K || ld_out < N || a_scale_row < 0 || a_scale_block < 0) return IFLB200_ERR_ARG;
+  const int es = out_dtype == IFLB200_F32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out) | (uintptr_t)ld_a |
+       (uintptr_t)ld_w | (uintptr_t)(ld_out * es)) & 15)
+    return IFLB200_ERR_ALIGN;
+  const int sms = device_sm_count();
+  if (sms == 0) return IFLB200_ERR_DEVICE;
+  BlockParams p = {};
+  p.M = M; p.N = N; p.K = K;
+  p.sa = a_scale; p.sa_row = a_scale_row; p.sa_block = a_scale_block;
+  p.sw = w_scale;
+  p.bias = bias; p.bias_dtype = bias_dtype;
+  p.out = reinterpret_cast<uint8_t*>(out);
+  p.ld_out = ld_out * es;
+  p.out_dtype = out_dtype;
+  p.early = M <= kEarlyWeightsMaxRows;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int steps = (K + kStep - 1) / kStep;
+  int form = g_form, bt = g_tokens, splits = g_splits;
+  if (form == 0) form = M <= 128 ? 1 : (M <= 512 ? 3 : 2);
+  if (bt == 0) {
+    const int most = form == 2 ? 256 : 128;
+    bt = M >= most ? most : (M + 15) / 16 * 16;
+  }
+  if (form == 1) {
+    const int64_t tiles = (int64_t)((M + bt - 1) / bt) * ((N + kStep - 1) / kStep);
+    if (splits == 0) {
+      splits = 1;
+      while (splits < 8 && tiles * splits * 2 <= sms && steps >= splits * 4) splits *= 2;
+    }
+    // a stage that is refilled while its accumulator waits needs a second one beside it
+    const int staging = out_dtype == IFLB200_F32 ? 2048 : 1024;
+    while (splits > 1 && (splits > steps || Layout<1, 2>::stages(bt, splits, staging) < 2)) splits /= 2;
+    return launch_form<1, 2>(a, ld_a, w, ld_w, p, bt, splits, sms, s);
+  }
+  if (form == 3) return launch_form<2, 2>(a, ld_a, w, ld_w, p, bt, 1, sms, s);
+  return launch_form<2, 1>(a, ld_a, w, ld_w, p, bt, 1, sms, s);
+}

@@ -121,6 +121,8 @@ __device__ unsigned int g_gemm_trace_cur;  // id of the launch whose block 0 is 
 #endif
 int set_stack_wait_budget_ns(uint64_t ns);  // stack_persistent.cu
 int set_peer_wait_budget_ns(uint64_t ns);   // xgpu_ops.cu
+int set_block_wait_budget_ns(uint64_t ns);  // gemm_block.cu
+int take_block_timeout_record(uint32_t* record, cudaStream_t s);
 
 __device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t rank) {
   uint32_t r;
@@ -2190,7 +2192,8 @@ extern "C" int iflb200_set_wait_budget_us(int64_t microseconds) {
   const uint64_t ns = microseconds ? (uint64_t)microseconds * 1000ull : kWaitBudgetNs;
   const cudaError_t e = cudaMemcpyToSymbol(g_gemm_wait_budget_ns, &ns, sizeof(ns));
   if (e != cudaSuccess) return (int)e;
-  const int st = set_stack_wait_budget_ns(ns);
+  int st = set_stack_wait_budget_ns(ns);
+  if (st == 0) st = set_block_wait_budget_ns(ns);
   return st != 0 ? st : set_peer_wait_budget_ns(ns);
 }
 
@@ -2216,7 +2219,11 @@ extern "C" int iflb200_gemm_take_timeout_record(uint32_t* record, void* stream) 
     if (e != cudaSuccess) return (int)e;
     e = cudaStreamSynchronize(s);
   }
-  return (int)e;
+  if (e != cudaSuccess) return (int)e;
+  uint32_t block = 0;
+  const int st = take_block_timeout_record(&block, s);
+  if (st == 0 && *record == 0) *record = block;
+  return st;
 }
 
 extern "C" int iflb200_gemm_fp8_raw(const void* a, int64_t ld_a, const void* w, int64_t ld_w, int M, int N,

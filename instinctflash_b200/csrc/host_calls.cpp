@@ -35,7 +35,7 @@ namespace {
   X(status_string) X(row_quant) X(quant_from_amax) X(dequant_rows) X(gated_act_quant) X(residual_norm_quant)    \
   X(residual_norm_quant_partials) X(qkv_split) X(wan_qkv) X(attn_combine_quant) X(gemm_fp8_raw)                 \
   X(gemm_fp8_partials) X(fp8_linear) X(fp8_linear_residual) X(fp8_linear_gated) X(pack_workspace_bytes)         \
-  X(dynamic_pack_bf16_e4m3) X(pack_bf16_e4m3)
+  X(dynamic_pack_bf16_e4m3) X(pack_bf16_e4m3) X(block_quant) X(block_linear) X(cache_append) X(cache_attention)
 
 struct Api {
 #define IFLB200_FIELD(name) decltype(&iflb200_##name) name = nullptr;
@@ -662,11 +662,199 @@ PyObject* guarded(PyObject* self, Args v, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------
+// Block scales: quantiser, linear, 8-bit cache
+// ------------------------------------------------------------------------------------------------
+constexpr int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+// [rows, cols] float32 with any non-negative strides; `written`: in one of the two orders that do not overlap
+const at::Tensor* block_scales(Call& c, PyObject* o, int64_t rows, int64_t cols, bool written) {
+  const at::Tensor* t = c.tensor(o);
+  if (!t) return nullptr;
+  c.ok = t->scalar_type() == ScalarType::Float && t->dim() == 2 && t->size(0) == rows && t->size(1) == cols && t->stride(0) >= 0 &&
+         t->stride(1) >= 0 &&
+         (!written || (t->stride(1) >= 1 && t->stride(0) >= t->stride(1) * cols) || (t->stride(0) >= 1 && t->stride(1) >= t->stride(0) * rows));
+  return c.ok ? t : nullptr;
+}
+
+PyObject* block_quant(PyObject*, Args v, Py_ssize_t nargs) {  // x, q, q_scale, act (-1: none)
+  ARITY(4);
+  Call c;
+  const int act = c.integer(v[3]);
+  if (!c.ok || act < -1 || act > 1) Py_RETURN_FALSE;
+  const Mat x = c.mat(v[0], kFloats);
+  if (!c.ok || (act >= 0 && x.cols % 2)) Py_RETURN_FALSE;
+  const int64_t K = act >= 0 ? x.cols / 2 : x.cols;
+  const Mat q = c.mat(v[1], kCodes, x.rows, K);
+  const at::Tensor* qs = c.ok ? block_scales(c, v[2], x.rows, blocks_of(K), true) : nullptr;
+  if (!qs || q.ld < K || x.ld < x.cols || !c.ready()) Py_RETURN_FALSE;
+  float* ps = qs->data_ptr<float>();
+  const int64_t s0 = qs->stride(0), s1 = qs->stride(1);
+  void* s = c.stream();
+  return finish("block_quant", [&] {
+    return api.block_quant(x.p, code_of(x.type), x.ld, (int)x.rows, (int)K, act, q.p, q.ld, ps, s0, s1, s);
+  });
+}
+
+PyObject* block_linear(PyObject*, Args v, Py_ssize_t nargs) {  // a, a_scale, w, w_scale, bias, out
+  ARITY(6);
+  Call c;
+  const Mat a = c.mat(v[0], kCodes), w = c.mat(v[2], kCodes), o = c.mat(v[5], kFloats, a.rows, w.rows);
+  if (!c.ok || !gemm_shapes(a, w)) Py_RETURN_FALSE;
+  const at::Tensor* as = block_scales(c, v[1], a.rows, blocks_of(a.cols), false);
+  const at::Tensor* ws = block_scales(c, v[3], blocks_of(w.rows), blocks_of(a.cols), false);
+  if (!as || !ws || !ws->is_contiguous()) Py_RETURN_FALSE;
+  void* bias = nullptr;
+  int bias_type = IFLB200_F32;
+  if (v[4] != Py_None) {
+    const at::Tensor* b = c.tensor(v[4]);
+    if (!b || (b->scalar_type() != ScalarType::Float && b->scalar_type() != ScalarType::BFloat16) || b->numel() != w.rows ||
+        !b->is_contiguous())
+      Py_RETURN_FALSE;
+    bias = b->data_ptr();
+    bias_type = code_of(b->scalar_type());
+  }
+  if (!c.ready()) Py_RETURN_FALSE;
+  const float *pa = as->data_ptr<float>(), *pw = ws->data_ptr<float>();
+  const int64_t s0 = as->stride(0), s1 = as->stride(1);
+  void* s = c.stream();
+  return finish("block_linear", [&] {
+    return api.block_linear(a.p, a.ld, w.p, w.ld, (int)a.rows, (int)w.rows, (int)a.cols, pa, s0, s1, pw, bias, bias_type, o.p,
+                            code_of(o.type), o.ld, s);
+  });
+}
+
+// [batch, tokens, heads, head_dim]
+struct HeadRows {
+  void* p = nullptr;
+  int64_t n[4] = {}, stride[3] = {};
+  ScalarType type = ScalarType::Undefined;
+};
+HeadRows head_rows(Call& c, PyObject* o, unsigned types) {
+  HeadRows h;
+  const at::Tensor* t = c.tensor(o);
+  if (!t) return h;
+  h.type = t->scalar_type();
+  c.ok = t->dim() == 4 && (types & bit(h.type)) && t->stride(3) == 1;
+  if (!c.ok) return h;
+  for (int i = 0; i < 4; ++i) {
+    h.n[i] = t->size(i);
+    c.ok = c.ok && h.n[i] <= INT32_MAX;
+    if (i < 3) h.stride[i] = t->stride(i);
+  }
+  h.p = t->data_ptr();
+  return h;
+}
+struct Cache {
+  void *k = nullptr, *v = nullptr;
+  float *ks = nullptr, *vs = nullptr;
+  int64_t pages = 0, heads = 0, page_tokens = 0, head_dim = 0;
+};
+Cache kv_cache(Call& c, Args v) {  // k, v, k_scale, v_scale
+  Cache x;
+  const at::Tensor* codes[2] = {c.tensor(v[0]), c.tensor(v[1])};
+  if (!c.ok) return x;
+  for (const at::Tensor* t : codes)
+    c.ok = c.ok && t->dim() == 4 && t->scalar_type() == ScalarType::Float8_e4m3fn && t->is_contiguous() && t->sizes() == codes[0]->sizes();
+  if (!c.ok) return x;
+  x.pages = codes[0]->size(0);
+  x.heads = codes[0]->size(1);
+  x.page_tokens = codes[0]->size(2);
+  x.head_dim = codes[0]->size(3);
+  const at::Tensor* s[2] = {block_scales(c, v[2], x.pages, x.heads, false), c.ok ? block_scales(c, v[3], x.pages, x.heads, false) : nullptr};
+  c.ok = c.ok && s[0]->is_contiguous() && s[1]->is_contiguous() && x.pages <= INT32_MAX && x.heads <= INT32_MAX &&
+         (x.head_dim == 64 || x.head_dim == 128 || x.head_dim == 256) && x.page_tokens >= 16 && x.page_tokens <= 256 && x.page_tokens % 16 == 0;
+  if (!c.ok) return x;
+  x.k = codes[0]->data_ptr();
+  x.v = codes[1]->data_ptr();
+  x.ks = s[0]->data_ptr<float>();
+  x.vs = s[1]->data_ptr<float>();
+  return x;
+}
+// int32 [n] contiguous, or null for None
+int32_t* ints(Call& c, PyObject* o, int64_t n) {
+  if (o == Py_None) return nullptr;
+  const at::Tensor* t = c.tensor(o);
+  if (!t) return nullptr;
+  c.ok = t->scalar_type() == ScalarType::Int && t->dim() == 1 && t->size(0) == n && (n <= 1 || t->stride(0) == 1);
+  return c.ok ? t->data_ptr<int32_t>() : nullptr;
+}
+struct Table {
+  int32_t* p = nullptr;
+  int64_t ld = 0, cols = 0;
+};
+Table page_table(Call& c, PyObject* o, int64_t batch) {
+  Table x;
+  const at::Tensor* t = c.tensor(o);
+  if (!t) return x;
+  c.ok = t->scalar_type() == ScalarType::Int && t->dim() == 2 && t->size(0) == batch && (t->size(1) <= 1 || t->stride(1) == 1) &&
+         t->size(1) <= INT32_MAX;
+  if (!c.ok) return x;
+  x.p = t->data_ptr<int32_t>();
+  x.ld = t->stride(0);
+  x.cols = t->size(1);
+  return x;
+}
+
+PyObject* cache_append(PyObject*, Args v, Py_ssize_t nargs) {  // cache k, v, k_scale, v_scale, k, v, table, start, counts
+  ARITY(9);
+  Call c;
+  const Cache x = kv_cache(c, v);
+  if (!c.ok) Py_RETURN_FALSE;
+  const HeadRows k = head_rows(c, v[4], kFloats), n = c.ok ? head_rows(c, v[5], kFloats) : HeadRows{};
+  if (!c.ok || k.type != n.type || !std::equal(k.n, k.n + 4, n.n) || k.n[2] != x.heads || k.n[3] != x.head_dim) Py_RETURN_FALSE;
+  const Table t = page_table(c, v[6], k.n[0]);
+  if (!c.ok || v[7] == Py_None) Py_RETURN_FALSE;
+  const int32_t *start = ints(c, v[7], k.n[0]), *counts = c.ok ? ints(c, v[8], k.n[0]) : nullptr;
+  if (!c.ready()) Py_RETURN_FALSE;
+  void* s = c.stream();
+  return finish("cache_append", [&] {
+    return api.cache_append(k.p, k.stride[0], k.stride[1], k.stride[2], n.p, n.stride[0], n.stride[1], n.stride[2], code_of(k.type),
+                            (int)k.n[0], (int)k.n[1], (int)x.heads, (int)x.head_dim, x.k, x.v, x.ks, x.vs, (int)x.pages,
+                            (int)x.page_tokens, t.p, t.ld, (int)t.cols, start, counts, s);
+  });
+}
+
+// q, cache k, v, k_scale, v_scale, table, lens, out, causal, prefix, softcap, slopes, scale, q_lens, workspace
+PyObject* cache_attention(PyObject*, Args v, Py_ssize_t nargs) {
+  ARITY(15);
+  Call c;
+  const HeadRows q = head_rows(c, v[0], bit(ScalarType::BFloat16) | bit(ScalarType::Half));
+  if (!c.ok) Py_RETURN_FALSE;
+  const Cache x = kv_cache(c, v + 1);
+  if (!c.ok || x.heads < 1 || q.n[2] < 1 || q.n[2] % x.heads || q.n[3] != x.head_dim) Py_RETURN_FALSE;
+  const Table t = page_table(c, v[5], q.n[0]);
+  if (!c.ok || v[6] == Py_None) Py_RETURN_FALSE;
+  const int32_t* lens = ints(c, v[6], q.n[0]);
+  if (!c.ok) Py_RETURN_FALSE;
+  const HeadRows o = head_rows(c, v[7], bit(q.type));
+  if (!c.ok || !std::equal(q.n, q.n + 4, o.n)) Py_RETURN_FALSE;
+  const int causal = c.flag(v[8]);
+  const int32_t* prefix = ints(c, v[9], q.n[0]);
+  const double cap = c.real(v[10]);
+  const float* slopes = c.ok && v[11] != Py_None ? c.f32(v[11], q.n[2]) : nullptr;
+  const double scale = c.ok && v[12] != Py_None ? c.real(v[12]) : 1.0 / std::sqrt((double)x.head_dim);
+  const int32_t* q_lens = c.ok ? ints(c, v[13], q.n[0]) : nullptr;
+  int64_t bytes = 0;
+  void* ws = c.ok ? c.vec(v[14], 0, ScalarType::Byte, &bytes) : nullptr;
+  if (!c.ok || (prefix && !causal) || !(cap >= 0.0) || reinterpret_cast<uintptr_t>(ws) % 16) Py_RETURN_FALSE;
+  if (v[11] != Py_None && THPVariable_Unpack(v[11]).numel() != q.n[2]) Py_RETURN_FALSE;
+  if (!c.ready()) Py_RETURN_FALSE;
+  void* s = c.stream();
+  return finish("cache_attention", [&] {
+    return api.cache_attention(q.p, code_of(q.type), q.stride[0], q.stride[1], q.stride[2], x.k, x.v, x.ks, x.vs, (int)x.pages,
+                               (int)x.page_tokens, (int)x.head_dim, t.p, t.ld, (int)t.cols, lens, q_lens, prefix, slopes,
+                               (int)q.n[0], (int)q.n[1], (int)q.n[2], (int)x.heads, (float)scale, (float)cap, causal, o.p,
+                               o.stride[0], o.stride[1], o.stride[2], ws, bytes, s);
+  });
+}
+
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&guarded<f>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     METHOD(gemm), METHOD(fp8_linear), METHOD(fp8_linear_residual), METHOD(fp8_linear_gated), METHOD(gemm_partials),
     METHOD(row_quant), METHOD(quant_from_amax), METHOD(dequant_rows), METHOD(gated_act_quant), METHOD(residual_norm_quant),
-    METHOD(qkv_split), METHOD(wan_qkv), METHOD(attn_combine), METHOD(dynamic_pack), METHOD(projection),
+    METHOD(qkv_split), METHOD(wan_qkv), METHOD(attn_combine), METHOD(block_quant), METHOD(block_linear),
+    METHOD(cache_append), METHOD(cache_attention), METHOD(dynamic_pack), METHOD(projection),
     {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
