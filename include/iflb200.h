@@ -359,8 +359,8 @@ IFLB200_API int iflb200_block_linear(const void* a, int64_t ld_a, const void* w,
                                      const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ld_out, void* stream);
 
 /*
- * Tuning: form of iflb200_block_linear (0 by rule, 1 single CTAs, 2 CTA pairs, 3 pairs with two K steps a stage), tokens
- * of a tile (0 by rule; a multiple of 16 up to 256, up to 128 for forms 1 and 3) and, for form 1, the CTAs that share a
+ * Tuning: form of iflb200_block_linear (0 by rule, 1 single CTAs, 2 CTA pairs), tokens
+ * of a tile (0 by rule; a multiple of 16 up to 128) and, for form 1, the CTAs that share a
  * tile's K range (0 by rule, up to 8).
  */
 IFLB200_API int iflb200_block_linear_set_form(int form, int tokens, int splits);

@@ -8,19 +8,26 @@
 // warps' registers (fp32 throughout), while the MMAs of the next step run into another accumulator.
 //
 // Weights are on the MMA's M side (128 rows a CTA: one row of weight blocks, so one weight scale a step), tokens on its
-// N side in tiles of any multiple of 16: the accumulator is the tile transposed.  Sixteen warps take it out in the
+// N side in tiles of any multiple of 16 up to 128: the accumulator is the tile transposed.  Sixteen warps take it out in the
 // 16 x 256-bit shape, where a thread holds four weight rows of two neighbouring tokens: one 8-byte read of the tokens'
 // scales serves four packed fused multiply-adds.
 //
 //   warp 0      TMA producer of W         warp 1   MMA issuer, tensor memory
-//   warp 2      TMA producer of A         warp 3   scales: sa * sw of the step into shared memory
-//   warps 4..19 promotion and epilogue
+//   warp 2      TMA producer of A         warp 3   scales: sa * sw into shared memory, eight K steps at a time
+//   warps 4..19 promotion and epilogue: a quadrant of tensor memory and 32 tokens each
 //
 // CG 2 works on CTA pairs (256 weight rows), CG 1 on single CTAs, whose K range a cluster of up to eight may share:
-// the partial sums meet in distributed shared memory and are added in the order of the ranges.  SL: K steps of a
-// stage; two of them share one commit where tiles are narrow (a commit occupies the issuing thread for 320 clocks).
+// the partial sums meet in distributed shared memory and are added in the order of the ranges.  A stage is two K steps
+// with an accumulator each, two stages fill tensor memory.
+//
+// What it took (4680 x 14336 x 5120, B200): 872 us with release semantics on the arrivals that free an accumulator in the
+// pair's other CTA (a memory barrier each), 568 without; 527 with a ring of scales in place of two steps'; 380 with
+// branch-free stages (the sums then stay in their registers) of two K steps.  The epilogue's work without the
+// sums takes 300, and a GEMM of the same size with one scale a row 240: both run at the 1000 W limit.
 #include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "../../include/iflb200.h"
 #include "launch.cuh"
@@ -35,6 +42,10 @@ constexpr int kEpi = 16;    // epilogue warps
 constexpr int kThreads = 32 * (4 + kEpi);
 constexpr uint64_t kBudgetNs = 2000000000ull;
 constexpr int kMaxStages = 8;
+constexpr int SL = 2;           // K steps of a stage
+constexpr int kAcc = 128;       // tensor-memory columns of an accumulator
+constexpr int kBatch = 8;       // K steps of a batch of scales; two batches in shared memory
+constexpr int kBars = 2 * kMaxStages + 2 + 4;
 constexpr int kMaxSmem = 227 * 1024;
 
 __device__ uint32_t g_record[4];
@@ -49,7 +60,8 @@ struct BlockParams {
   uint32_t idesc;
   const float* sa;
   int64_t sa_row, sa_block;
-  const float* sw;                       // [ceil(N / 128)][num_k]
+  int blocks;                            // of K; num_k: rounded up to whole stages
+  const float* sw;                       // [ceil(N / 128)][blocks]
   const void* bias;
   int bias_dtype;
   uint8_t* out;
@@ -59,11 +71,15 @@ struct BlockParams {
   int early;                             // the first weights may be read ahead of the dependency wait
 };
 
-__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr)
-               : "memory");
+// Thirty-two token columns of sixteen lanes: r[4 j + {0, 1}] = weight row t/4, tokens 8 j + 2 (t % 4) + {0, 1};
+// r[4 j + {2, 3}] = row t/4 + 8.
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 __device__ __forceinline__ void store_transposed(uint32_t addr, const uint32_t (&v)[4]) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]),
@@ -92,6 +108,18 @@ __device__ __forceinline__ void st_cluster_64x2(uint32_t addr, uint32_t rank, ui
       : "memory");
 }
 
+// Arrival at the leader's barrier.  It publishes no memory: what it stands for is that tensor memory has been read, which the
+// tcgen05 fence ahead of it orders.  (With release semantics at cluster scope it is a memory barrier, which the epilogue warps
+// waited for longer than for anything else.)
+__device__ __forceinline__ void arrive_relaxed_cluster(uint32_t bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [ra];\n\t}"
+      ::"r"(bar), "r"(rank)
+      : "memory");
+}
+
 // Bounded wait of one thread; false once the CTA gives up.
 __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t code) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -111,7 +139,7 @@ __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile
     }
   }
 }
-// The same for a converged warp.
+// wait_one for a converged warp.
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t code) {
   if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
   const bool ok = wait_one(bar, parity, abort, code);
@@ -119,22 +147,22 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatil
 }
 
 __device__ __forceinline__ uint32_t pair_bf16(float a, float b) {
-  return f32_to_bf16_bits(a) | (f32_to_bf16_bits(b) << 16);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t pair_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int CG, int SL>
+template <int CG>
 struct Layout {
-  static constexpr int kAcc = 256 / SL;                     // tensor-memory columns of an accumulator: two stages of SL
-  static constexpr int kScales = 2 * SL * kAcc * 4;         // bytes
+  static constexpr int kScales = 2 * kBatch * kAcc * 4;  // bytes
   __host__ __device__ static int slab(int bt) { return kStep * kStep + bt / CG * kStep; }
   static int blocks_of(int bt, int splits) { return (bt / 16 + splits - 1) / splits; }  // token blocks that a rank adds up
   static int meeting(int bt, int splits) { return splits > 1 ? blocks_of(bt, splits) * splits * 4 * 2048 : 0; }
   static int fixed(int bt, int splits, int staging) {
-    return 1024 + kEpi * staging + kScales + meeting(bt, splits) + (2 * kMaxStages + 8) * 8 + 16;
+    return 1024 + kEpi * staging + kScales + meeting(bt, splits) + kBars * 8 + 16;
   }
   static int stages(int bt, int splits, int staging) {
     const int n = (kMaxSmem - fixed(bt, splits, staging)) / (SL * slab(bt));
@@ -142,11 +170,11 @@ struct Layout {
   }
 };
 
-template <int CG, int SL>
+template <int CG>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_constant__ CUtensorMap tm_w,
                       const __grid_constant__ BlockParams p) {
-  using L = Layout<CG, SL>;
+  using L = Layout<CG>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -161,9 +189,9 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_con
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto done_bar = [&](int s) { return bar0 + 8u * (kMaxStages + s); };      // MMAs of the stage complete: slabs free, accumulators full
   auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kMaxStages + a); };
-  auto sfull_bar = [&](int a) { return bar0 + 8u * (2 * kMaxStages + 2 + a); };
-  auto sempty_bar = [&](int a) { return bar0 + 8u * (2 * kMaxStages + 4 + a); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar0 - base) + (2 * kMaxStages + 8) * 8);
+  auto sfull_bar = [&](int i) { return bar0 + 8u * (2 * kMaxStages + 2 + i); };
+  auto sempty_bar = [&](int i) { return bar0 + 8u * (2 * kMaxStages + 4 + i); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar0 - base) + kBars * 8);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -172,9 +200,9 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_con
   const int splits = CG == 1 ? p.splits : 1;
   const int width = CG == 1 ? splits : 2;
   const int first_unit = blockIdx.x / width, unit_stride = gridDim.x / width;
-  // this CTA's K range, in blocks
-  const int kb0 = CG == 1 ? (int)((int64_t)p.num_k * rank / splits) : 0;
-  const int kb1 = CG == 1 ? (int)((int64_t)p.num_k * (rank + 1) / splits) : p.num_k;
+  // this CTA's K range, in blocks: whole stages (past the operands' last columns TMA reads zeros)
+  const int kb0 = CG == 1 ? (int)((int64_t)(p.num_k / SL) * rank / splits) * SL : 0;
+  const int kb1 = CG == 1 ? (int)((int64_t)(p.num_k / SL) * (rank + 1) / splits) * SL : p.num_k;
   auto place = [&](int unit, int& t_blk, int& w_blk) {
     const int band = p.group_m * p.num_n, g = unit / band;
     const int first = g * p.group_m, size = min(p.num_m - first, p.group_m), r = unit - g * band;
@@ -215,7 +243,6 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_con
   const uint32_t tmem_base = *tmem_slot;
   cluster_wait();
 
-  uint64_t acc[4][8];  // sums of the epilogue warps: token block, then half * 4 + group of 8 tokens * 2 + row of 8
   const int quad = warp & 3, part = (warp - 4) >> 2;
   const int r4 = lane >> 2, c4 = lane & 3;
 
@@ -234,12 +261,12 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_con
         for (int kb = kb0; kb < kb1; kb += SL) {
           ok = wait_one(done_bar(stage), phase ^ 1, abort_flag, (1u << 24) | (1u << 16) | (uint32_t)(kb & 0xFFFF));
           if (!ok) break;
-          const int slabs = min(SL, kb1 - kb);
           const uint32_t bar = full_bar(stage), dst = base + stage * SL * slab_bytes + (weights ? 0u : w_bytes);
-          if (leader) mbar_arrive_expect_tx(bar, (uint32_t)(CG * slabs) * (weights ? w_bytes : t_bytes));
+          if (leader) mbar_arrive_expect_tx(bar, (uint32_t)(CG * SL) * (weights ? w_bytes : t_bytes));
           if (!waited) grid_dependency_wait();
           waited = true;
-          for (int h = 0; h < slabs; ++h) {
+#pragma unroll
+          for (int h = 0; h < SL; ++h) {
             const int x = (kb + h) * kStep;
             if (CG == 2) {
               tma_load_2d_pair(dst + h * slab_bytes, weights ? &tm_w : &tm_t, bar & kPeerBitMask, x, weights ? w_row : t_row);
@@ -273,10 +300,10 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_con
                wait_one(full_bar(stage), phase, abort_flag, (2u << 24) | (3u << 16) | (it & 0xFFFF));
           if (!ok) break;
           tc_fence_after();
-          const int slabs = min(SL, kb1 - kb);
-          for (int h = 0; h < slabs; ++h) {
+#pragma unroll
+          for (int h = 0; h < SL; ++h) {
             const uint64_t at = (uint64_t)(((stage * SL + h) * slab_bytes) >> 4);
-            const uint32_t d = tmem_base + (a * SL + h) * L::kAcc;
+            const uint32_t d = tmem_base + (a * SL + h) * kAcc;
 #pragma unroll
             for (int j = 0; j < kStep / 32; ++j) {
               if (CG == 2) mma_f8f6f4_pair(d, dw0 + at + 2 * j, dt0 + at + 2 * j, p.idesc, j > 0);
@@ -295,56 +322,46 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_con
     __syncwarp();
   } else if (warp == 3) {
     // ------------------------------------------------------------------ scales
-    // Read in batches of several steps, 32 values a lane in flight: one trip to L2 a batch.
-    constexpr int TPL = L::kAcc / 32, BATCH = 32 / TPL;
+    // 32 values a lane in flight: one trip to L2 for eight K steps.
+    constexpr int TPL = kAcc / 32;
     bool ok = true;
-    uint32_t it = 0;
+    uint32_t batch = 0;
     grid_dependency_wait();
     for (int unit = first_unit; ok && unit < p.units; unit += unit_stride) {
       int t_blk, w_blk;
       place(unit, t_blk, w_blk);
       const int nb = min(w_blk * CG + (CG == 2 ? (int)rank : 0), (p.N - 1) / kStep);
-      const float* sw = p.sw + (int64_t)nb * p.num_k;
-      const float* sa[TPL];
+      const float* sw = p.sw + (int64_t)nb * p.blocks;
+      for (int kb = kb0; kb < kb1; kb += kBatch, ++batch) {
+        float v[kBatch][TPL];
 #pragma unroll
-      for (int i = 0; i < TPL; ++i) sa[i] = p.sa + (int64_t)min(t_blk * p.bt + 32 * i + lane, p.M - 1) * p.sa_row;
-      for (int kb = kb0; ok && kb < kb1; kb += BATCH) {
-        float v[BATCH][TPL], w[BATCH];
+        for (int i = 0; i < TPL; ++i) {
+          const float* sa = p.sa + (int64_t)min(t_blk * p.bt + 32 * i + lane, p.M - 1) * p.sa_row + (int64_t)kb * p.sa_block;
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          w[j] = kb + j < kb1 ? __ldg(sw + kb + j) : 0.0f;
-#pragma unroll
-          for (int i = 0; i < TPL; ++i)
-            v[j][i] = kb + j < kb1 && 32 * i + lane < p.bt ? __ldg(sa[i] + (int64_t)(kb + j) * p.sa_block) : 0.0f;
+          for (int j = 0; j < kBatch; ++j) v[j][i] = kb + j < p.blocks && 32 * i < p.bt ? __ldg(sa + j * p.sa_block) : 0.0f;
         }
+        const float w = lane < kBatch && kb + lane < p.blocks ? __ldg(sw + kb + lane) : 0.0f;
+        const uint32_t half = batch & 1u;
+        ok = wait_warp(sempty_bar(half), ((batch >> 1) & 1u) ^ 1u, abort_flag, (4u << 24) | (5u << 16) | (batch & 0xFFFF));
+        if (!ok) break;
 #pragma unroll
-        for (int s = 0; s < BATCH / SL; ++s) {
-          if (ok && kb + s * SL < kb1) {
-            const uint32_t a = it & 1u;
-            ok = wait_warp(sempty_bar(a), ((it >> 1) & 1u) ^ 1u, abort_flag, (4u << 24) | (5u << 16) | (it & 0xFFFF));
-            if (ok) {
+        for (int j = 0; j < kBatch; ++j) {
+          const float wj = __shfl_sync(0xFFFFFFFFu, w, j);
 #pragma unroll
-              for (int h = 0; h < SL; ++h) {
-#pragma unroll
-                for (int i = 0; i < TPL; ++i)
-                  sts32(scales0 + ((a * SL + h) * L::kAcc + 32 * i + lane) * 4, v[s * SL + h][i] * w[s * SL + h]);
-              }
-              __syncwarp();
-              if (lane == 0) mbar_arrive(sfull_bar(a));
-              ++it;
-            }
-          }
+          for (int i = 0; i < TPL; ++i) sts32(scales0 + ((half * kBatch + j) * kAcc + 32 * i + lane) * 4, v[j][i] * wj);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sfull_bar(half));
       }
     }
   } else {
     // ------------------------------------------------------------------ promotion, epilogue
     bool ok = true;
     int stage = 0;
-    uint32_t phase = 0, it = 0;
+    uint32_t phase = 0, it = 0, batch = 0;
     const uint32_t staging = staging0 + (uint32_t)(warp - 4) * p.staging;
     // bias and stores of one block of 16 tokens
-    auto store = [&](const uint64_t (&s)[8], int tok, int n0, const float (&bs)[4]) {
+    auto store = [&](const uint64_t* s, int tok, int n0, const float (&bs)[4]) {
       __syncwarp();  // the block before this one has left the staging buffer
       if (p.out_dtype == IFLB200_F32) {
         // 128-byte rows of 32 columns, 16-byte pieces swizzled by the token
@@ -411,66 +428,82 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_con
                                                 : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[n]);
         }
       }
+      // sums: block of 16 tokens, then half of the lanes * 4 + eight tokens * 2 + row of 8
+      uint64_t acc[2][8];
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int i = 0; i < 16; ++i) acc[i >> 3][i & 7] = 0;
+      // A warp whose tokens are all past the tile's end only keeps the barriers in step.  (A loop of its own, and no branch in
+      // the other's body: there the compiler moves the sums from register to register on every path.)
+      auto step = [&](auto active) {
+        for (int kb = kb0; kb < kb1; kb += SL, ++it) {
+          const uint32_t a = it & 1u;
+          const int in_batch = (kb - kb0) & (kBatch - 1);
+          if (in_batch == 0)
+            ok = wait_warp(sfull_bar(batch & 1u), (batch >> 1) & 1u, abort_flag, (3u << 24) | (6u << 16) | (it & 0xFFFF));
+          ok = ok && wait_warp(done_bar(stage), phase, abort_flag, (3u << 24) | (4u << 16) | (it & 0xFFFF));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t t_acc = tmem_base + ((uint32_t)(quad * 32) << 16) + a * SL * kAcc + 32 * part;
+          const uint32_t s_at = scales0 + (((batch & 1u) * kBatch + in_batch) * kAcc + 32 * part + 2 * c4) * 4;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[b][i] = 0;
-      for (int kb = kb0; kb < kb1; kb += SL, ++it) {
-        const uint32_t a = it & 1u;
-        ok = wait_warp(sfull_bar(a), (it >> 1) & 1u, abort_flag, (3u << 24) | (6u << 16) | (it & 0xFFFF)) &&
-             wait_warp(done_bar(stage), phase, abort_flag, (3u << 24) | (4u << 16) | (it & 0xFFFF));
-        if (!ok) break;
-        tc_fence_after();
-        const int slabs = min(SL, kb1 - kb);
+          for (int h = 0; h < SL; ++h) {
+            // (tokens past the tile's end inside a group are taken too: their sums are never stored)
+            uint32_t r[2][16];
+            uint64_t sc[4];
+            if constexpr (decltype(active)::value) {
+              tmem_ld_32(t_acc + h * kAcc, r[0]);
+              tmem_ld_32(t_acc + h * kAcc + (16u << 16), r[1]);
 #pragma unroll
-        for (int h = 0; h < SL; ++h) {
-          if (h < slabs) {
-            const uint32_t t_acc = tmem_base + ((uint32_t)(quad * 32) << 16) + (a * SL + h) * L::kAcc;
-            const uint32_t s_at = scales0 + ((a * SL + h) * L::kAcc + 2 * c4) * 4;
-#pragma unroll
-            for (int b = 0; b < (SL == 1 ? 4 : 2); ++b) {
-              const int block = part + 4 * b;
-              if (block < blocks) {
-                uint32_t r[16];
-                tmem_ld_16(t_acc + 16 * block, r);
-                tmem_ld_16(t_acc + (16u << 16) + 16 * block, r + 8);
-                const uint64_t s0 = lds64(s_at + 64 * block), s1 = lds64(s_at + 64 * block + 32);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  acc[b][i] = fma2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), (i >> 1) & 1 ? s1 : s0, acc[b][i]);
+              for (int j = 0; j < 4; ++j) sc[j] = lds64(s_at + (h * kAcc + 8 * j) * 4);
+              tmem_ld_wait();
+            }
+            if (h == SL - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                if (CG == 2) arrive_relaxed_cluster(tempty_bar(a), 0);
+                else mbar_arrive(tempty_bar(a));
               }
             }
+            if constexpr (decltype(active)::value) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)  // i: eight tokens * 2 + row of 8
+                  acc[i >> 2][half * 4 + (i & 3)] = fma2(pack2(__uint_as_float(r[half][2 * i]), __uint_as_float(r[half][2 * i + 1])),
+                                                         sc[i >> 1], acc[i >> 2][half * 4 + (i & 3)]);
+            }
+          }
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+          if (in_batch + SL == kBatch || kb + SL >= kb1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sempty_bar(batch & 1u));
+            ++batch;
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (CG == 2) mbar_arrive_cluster(tempty_bar(a), 0);
-          else mbar_arrive(tempty_bar(a));
-          mbar_arrive(sempty_bar(a));
-        }
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
-        }
-      }
+      };
+      if (32 * part < p.bt) step(std::true_type());
+      else step(std::false_type());
       if (!ok) break;
       if (CG == 1 && splits > 1) {
         // to the rank that adds the block up: [own block][source rank][quadrant][piece][lane]
 #pragma unroll
-        for (int b = 0; b < (SL == 1 ? 4 : 2); ++b) {
-          const int block = part + 4 * b;
+        for (int b = 0; b < 2; ++b) {
+          const int block = 2 * part + b;
           if (block < blocks) {
             const uint32_t at = meeting0 + (uint32_t)(((block / splits) * splits + (int)rank) * 4 + quad) * 2048 + lane * 16;
+            const uint64_t* v = acc[b];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) st_cluster_64x2(at + i * 512, (uint32_t)(block % splits), acc[b][2 * i], acc[b][2 * i + 1]);
+            for (int i = 0; i < 4; ++i) st_cluster_64x2(at + i * 512, (uint32_t)(block % splits), v[2 * i], v[2 * i + 1]);
           }
         }
       } else {
 #pragma unroll
-        for (int b = 0; b < (SL == 1 ? 4 : 2); ++b) {
-          const int block = part + 4 * b;
+        for (int b = 0; b < 2; ++b) {
+          const int block = 2 * part + b;
           if (block < blocks) store(acc[b], tok_base + 16 * block, n0, bs);
         }
       }
@@ -572,15 +605,15 @@ int operand_map(CUtensorMap* tm, const void* ptr, int rows, int K, int64_t ld, i
 // iflb200_block_linear_set_form; zeros: by rule
 int g_form = 0, g_tokens = 0, g_splits = 0;
 
-template <int CG, int SL>
+template <int CG>
 int launch_form(const void* a, int64_t ld_a, const void* w, int64_t ld_w, BlockParams p, int bt, int splits, int sms, cudaStream_t s) {
-  using L = Layout<CG, SL>;
+  using L = Layout<CG>;
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return IFLB200_ERR_DEVICE;
   if (!attr_set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_block_kernel<CG, SL>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_block_kernel<CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
     if (e != cudaSuccess) return (int)e;
     attr_set[dev] = true;
   }
@@ -588,7 +621,8 @@ int launch_form(const void* a, int64_t ld_a, const void* w, int64_t ld_w, BlockP
   p.splits = splits;
   p.num_m = (p.M + bt - 1) / bt;
   p.num_n = (p.N + CG * kStep - 1) / (CG * kStep);
-  p.num_k = (p.K + kStep - 1) / kStep;
+  p.blocks = (p.K + kStep - 1) / kStep;
+  p.num_k = (p.blocks + SL - 1) / SL * SL;
   p.units = p.num_m * p.num_n;
   p.group_m = p.num_m <= 24 ? p.num_m : 16;
   p.staging = p.out_dtype == IFLB200_F32 ? 2048 : 1024;
@@ -601,7 +635,7 @@ int launch_form(const void* a, int64_t ld_a, const void* w, int64_t ld_w, BlockP
   const int most = CG == 2 ? sms / 2 : sms;
   const unsigned ctas = CG == 1 && splits > 1 ? (unsigned)(p.units * splits) : (unsigned)(CG * (p.units < most ? p.units : most));
   const size_t smem = (size_t)L::fixed(bt, splits, p.staging) + (size_t)p.stages * SL * L::slab(bt);
-  const cudaError_t e = launch_dep(gemm_fp8_block_kernel<CG, SL>, dim3(ctas), dim3(kThreads), smem, s, CG == 2 ? 2 : splits,
+  const cudaError_t e = launch_dep(gemm_fp8_block_kernel<CG>, dim3(ctas), dim3(kThreads), smem, s, CG == 2 ? 2 : splits,
                                    dependent_launch_for(p.M, true), tt, tw, p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
@@ -630,8 +664,7 @@ int take_block_timeout_record(uint32_t* record, cudaStream_t s) {
 using namespace iflb200;
 
 extern "C" int iflb200_block_linear_set_form(int form, int tokens, int splits) {
-  if (form < 0 || form > 3 || tokens < 0 || tokens > 256 || tokens % 16 || splits < 0 || splits > 8) return IFLB200_ERR_ARG;
-  if (form != 2 && tokens > 128) return IFLB200_ERR_ARG;  // forms of two K steps a stage
+  if (form < 0 || form > 2 || tokens < 0 || tokens > kAcc || tokens % 16 || splits < 0 || splits > 8) return IFLB200_ERR_ARG;
   if (form != 1 && splits > 1) return IFLB200_ERR_ARG;
   g_form = form;
   g_tokens = tokens;
@@ -666,24 +699,18 @@ extern "C" int iflb200_block_linear(const void* a, int64_t ld_a, const void* w, 
   p.out_dtype = out_dtype;
   p.early = M <= kEarlyWeightsMaxRows;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int steps = (K + kStep - 1) / kStep;
+  const int steps = (K + SL * kStep - 1) / (SL * kStep);  // stages
   int form = g_form, bt = g_tokens, splits = g_splits;
-  if (form == 0) form = M <= 128 ? 1 : (M <= 512 ? 3 : 2);
-  if (bt == 0) {
-    const int most = form == 2 ? 256 : 128;
-    bt = M >= most ? most : (M + 15) / 16 * 16;
+  if (form == 0) form = M <= 128 ? 1 : 2;
+  if (bt == 0) bt = M >= kAcc ? kAcc : (M + 15) / 16 * 16;
+  if (form == 2) return launch_form<2>(a, ld_a, w, ld_w, p, bt, 1, sms, s);
+  const int64_t tiles = (int64_t)((M + bt - 1) / bt) * ((N + kStep - 1) / kStep);
+  if (splits == 0) {
+    splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= sms && steps >= splits * 2) splits *= 2;
   }
-  if (form == 1) {
-    const int64_t tiles = (int64_t)((M + bt - 1) / bt) * ((N + kStep - 1) / kStep);
-    if (splits == 0) {
-      splits = 1;
-      while (splits < 8 && tiles * splits * 2 <= sms && steps >= splits * 4) splits *= 2;
-    }
-    // a stage that is refilled while its accumulator waits needs a second one beside it
-    const int staging = out_dtype == IFLB200_F32 ? 2048 : 1024;
-    while (splits > 1 && (splits > steps || Layout<1, 2>::stages(bt, splits, staging) < 2)) splits /= 2;
-    return launch_form<1, 2>(a, ld_a, w, ld_w, p, bt, splits, sms, s);
-  }
-  if (form == 3) return launch_form<2, 2>(a, ld_a, w, ld_w, p, bt, 1, sms, s);
-  return launch_form<2, 1>(a, ld_a, w, ld_w, p, bt, 1, sms, s);
+  // a stage that is refilled while its accumulator waits needs a second one beside it
+  const int staging = out_dtype == IFLB200_F32 ? 2048 : 1024;
+  while (splits > 1 && (splits > steps || Layout<1>::stages(bt, splits, staging) < 2)) splits /= 2;
+  return launch_form<1>(a, ld_a, w, ld_w, p, bt, splits, sms, s);
 }

@@ -76,9 +76,9 @@ def test_entry_points_reject_bad_arguments_before_any_launch():
     assert linear(sa=None) == -1 and linear(sw=None) == -1 and linear(lda=128) == -1 and linear(ldo=32) == -1 and linear(b=-4) == -1
     assert linear(dt=7) == -4 and linear(bias=p, bt=2) == -4
 
-    for ok in ((0, 0, 0), (1, 128, 8), (2, 256, 1), (3, 16, 0)):
+    for ok in ((0, 0, 0), (1, 128, 8), (2, 128, 1), (2, 16, 0)):
         assert lib.iflb200_block_linear_set_form(*ok) == 0
-    for bad in ((4, 0, 0), (1, 256, 0), (2, 24, 0), (3, 0, 2), (1, 0, 9), (-1, 0, 0)):
+    for bad in ((3, 0, 0), (1, 144, 0), (2, 24, 0), (2, 0, 2), (1, 0, 9), (-1, 0, 0)):
         assert lib.iflb200_block_linear_set_form(*bad) == -1
     assert lib.iflb200_block_linear_set_form(0, 0, 0) == 0
 
