@@ -399,6 +399,11 @@ IFLB200_API int iflb200_cache_attention(const void* q, int dtype, int64_t q_b, i
                                         int64_t workspace_bytes, void* stream);
 
 /*
+ * Tuning: form of iflb200_cache_attention (0 by rule, 1 few rows, 2 row tiles on tcgen05).
+ */
+IFLB200_API int iflb200_cache_attention_set_form(int form);
+
+/*
  * Per-tensor dynamic e4m3 pack (the torch-FP8-linear recipe):
  *   amax = max |x| (NaN propagates);  scale = max(amax, 1e-12) * fp32(1/448);
  *   q = e4m3_rn(clamp(x / scale, -448, 448))   (IEEE division, NaN propagates)

@@ -60,6 +60,7 @@ SIGNATURES = {
                                   _p, _p]),
     "iflb200_cache_attention": (_i, [_p, _i, _l, _l, _l, _p, _p, _p, _p, _i, _i, _i, _p, _l, _i, _p, _p, _p, _p, _i, _i, _i,
                                      _i, _f, _f, _i, _p, _l, _l, _l, _p, _l, _p]),
+    "iflb200_cache_attention_set_form": (_i, [_i]),
     "iflb200_pack_workspace_bytes": (_z, [_l]),
     "iflb200_dynamic_pack_bf16_e4m3": (_i, [_p, _l, _p, _p, _p, _z, _p]),
     "iflb200_dynamic_pack_bf16_e4m3_noalloc": (_i, [_p, _l, _p, _p, _p]),

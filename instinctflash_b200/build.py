@@ -28,6 +28,7 @@ SOURCES = (("gemm_fp8_sm100.cu", (), "gemm_fp8_sm100"),
            ("block_ops.cu", (), "block_ops"),
            ("gemm_block.cu", (), "gemm_block"),
            ("cache_attn.cu", (), "cache_attn"),
+           ("cache_attn_tiles.cu", (), "cache_attn_tiles"),
            ("row_ops.cu", ("-DIFLB200_ROW_PART=0",), "row_ops_quant"),
            ("row_ops.cu", ("-DIFLB200_ROW_PART=1",), "row_ops_gated_pack"),
            ("row_ops.cu", ("-DIFLB200_ROW_PART=2",), "row_ops_resnorm"))

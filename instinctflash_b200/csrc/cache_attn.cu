@@ -5,44 +5,15 @@
 //
 // Every mask here leaves a row the keys below a limit of its own: the sequence's length, or with a causal mask
 // max(position + 1, prefix).
-#include <cuda_runtime.h>
-
-#include "../../include/iflb200.h"
-#include "launch.cuh"
-#include "rowmath.cuh"
+#include "cache_attn.cuh"
 
 namespace iflb200 {
 
 namespace {
 
-struct AttendArgs {
-  const void* q;
-  int64_t q_b, q_t, q_h;
-  void* out;
-  int64_t o_b, o_t, o_h;
-  const uint8_t* k;
-  const uint8_t* v;
-  const float* ks;
-  const float* vs;
-  const int32_t* table;
-  int64_t ld_table;
-  const int32_t* lens;
-  const int32_t* q_lens;
-  const int32_t* prefix;
-  const float* slopes;
-  float scale, cap;
-  int B, T, HQ, H, G, P, pages, max_pages, causal;
-  int row_tiles, chunk, splits;     // keys of a chunk; most chunks a sequence can have
-  uint32_t* tickets;                // one for each (sequence, head and row tile), zero between calls
-  float* partial;                   // [ticket][chunk][rows][D], then [ticket][chunk][rows][2]
-  int64_t partial_ml;               // floats ahead of the second part
-};
-
 constexpr int kWarps = 4;
 constexpr int kTile = 32;    // keys a warp takes at a time
 constexpr int kStages = 3;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 5.0f;  // base-2 exponent by which a score may pass the running maximum before it moves
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -57,12 +28,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
-// Two e4m3 codes in the low half of `two` as two f16 (exact).
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
-  return r;
-}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -72,10 +37,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // 1.0 in each half of x that is a NaN (all bits below the sign set: what a NaN code converts to), else 0.
 __device__ __forceinline__ uint32_t nan_halves(uint32_t x) {
   return ((x & 0x7FFF) > 0x7C00 ? 0x3C00u : 0u) | ((x & 0x7FFF0000u) > 0x7C000000u ? 0x3C000000u : 0u);
@@ -83,21 +44,6 @@ __device__ __forceinline__ uint32_t nan_halves(uint32_t x) {
 __device__ __forceinline__ uint32_t without_nan(uint32_t x) {
   return ((x & 0x7FFF) > 0x7C00 ? 0u : x & 0xFFFF) | ((x & 0x7FFF0000u) > 0x7C000000u ? 0u : x & 0xFFFF0000u);
 }
-
-// cap * tanh(s / cap).  tanh(x) = 1 - 2 / (1 + e^2x) is off by 1e-7 of 1; near zero, where that is more than fp32 keeps
-// of the result, the series (next term below 1e-7 of x at 1/4).
-__device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap) {
-  const float x = s * inv_cap;
-  const float y = x * x;
-  const float near = x + x * y * (-0.33333333f + y * (0.13333333f + y * (-0.053968254f + y * 0.021869489f)));
-  const float far = 1.0f - 2.0f * rcp_approx_ftz(1.0f + ex2_approx_ftz(2.0f * kLog2e * x));
-  return cap * (fabsf(x) < 0.25f ? near : far);
-}
-
-__device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 
 // ---------------------------------------------------------------------------------------------
 // Few rows (query token x head of a group): bound by the cache's bytes.
@@ -502,10 +448,15 @@ int launch_rows(const AttendArgs& a, cudaStream_t s) {
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
+// iflb200_cache_attention_set_form; 0: by rule
+int g_form = 0;
+constexpr int64_t kFewRows = 32;
+
 template <typename T>
 int attend(AttendArgs a, int D, void* workspace, int64_t bytes, cudaStream_t s) {
   const int64_t rows = (int64_t)a.T * a.G;
-  const int nt = D == 256 || rows <= 8 ? 1 : 2, per = 8 * nt;
+  const bool many = g_form == 2 || (g_form == 0 && rows > kFewRows);
+  const int nt = D == 256 || rows <= 8 ? 1 : 2, per = many ? attend_tiles_rows(D) : 8 * nt;
   const int64_t tiles = (rows + per - 1) / per;
   if (tiles * a.H > 65535) return IFLB200_ERR_SHAPE;
   a.row_tiles = (int)tiles;
@@ -514,7 +465,7 @@ int attend(AttendArgs a, int D, void* workspace, int64_t bytes, cudaStream_t s) 
   // Chunks of keys: enough for two waves of CTAs, none shorter than a step of all warps, as many as the workspace takes.
   const int64_t keys = (int64_t)a.max_pages * a.P, units = (int64_t)a.B * a.H * tiles;
   constexpr int64_t kLeast = kWarps * kTile;
-  const int64_t want = (4ll * sms + units - 1) / units;
+  const int64_t want = ((many ? 1ll : 4ll) * sms + units - 1) / units;
   // The tickets have a place of their own whatever the geometry: they are zero between calls, partial results are not.
   // (Sequences are only shared where there are fewer units than CTAs wanted.)
   constexpr int64_t head = 4096;
@@ -531,6 +482,7 @@ int attend(AttendArgs a, int D, void* workspace, int64_t bytes, cudaStream_t s) 
   a.tickets = reinterpret_cast<uint32_t*>(workspace);
   a.partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + head);
   a.partial_ml = units * a.splits * per * D;
+  if (many) return launch_attend_tiles<T>(a, D, s);
   if (D == 64) return nt == 1 ? launch_rows<64, 1, T>(a, s) : launch_rows<64, 2, T>(a, s);
   if (D == 128) return nt == 1 ? launch_rows<128, 1, T>(a, s) : launch_rows<128, 2, T>(a, s);
   return launch_rows<256, 1, T>(a, s);
@@ -541,6 +493,12 @@ int attend(AttendArgs a, int D, void* workspace, int64_t bytes, cudaStream_t s) 
 }  // namespace iflb200
 
 using namespace iflb200;
+
+extern "C" int iflb200_cache_attention_set_form(int form) {
+  if (form < 0 || form > 2) return IFLB200_ERR_ARG;
+  g_form = form;
+  return IFLB200_OK;
+}
 
 extern "C" int iflb200_cache_attention(const void* q, int dtype, int64_t q_b, int64_t q_t, int64_t q_h, const void* k_codes,
                                        const void* v_codes, const float* k_scale, const float* v_scale, int pages,

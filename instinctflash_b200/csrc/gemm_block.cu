@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "../../include/iflb200.h"
+#include "bounded_wait.cuh"
 #include "launch.cuh"
 #include "rowmath.cuh"
 
@@ -40,16 +41,12 @@ namespace {
 constexpr int kStep = 128;  // bytes of K and weight rows: a block of the weight
 constexpr int kEpi = 16;    // epilogue warps
 constexpr int kThreads = 32 * (4 + kEpi);
-constexpr uint64_t kBudgetNs = 2000000000ull;
 constexpr int kMaxStages = 8;
 constexpr int SL = 2;           // K steps of a stage
 constexpr int kAcc = 128;       // tensor-memory columns of an accumulator
 constexpr int kBatch = 8;       // K steps of a batch of scales; two batches in shared memory
 constexpr int kBars = 2 * kMaxStages + 2 + 4;
 constexpr int kMaxSmem = 227 * 1024;
-
-__device__ uint32_t g_record[4];
-__device__ uint64_t g_budget_ns = kBudgetNs;
 
 struct BlockParams {
   int M, N, K;
@@ -118,32 +115,6 @@ __device__ __forceinline__ void arrive_relaxed_cluster(uint32_t bar, uint32_t ra
       "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [ra];\n\t}"
       ::"r"(bar), "r"(rank)
       : "memory");
-}
-
-// Bounded wait of one thread; false once the CTA gives up.
-__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t code) {
-  if (mbar_try_wait(bar, parity)) return true;
-  uint64_t t0 = 0;
-  uint32_t spins = 0;
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort) return false;
-    if (++spins > 2048) {
-      if (t0 == 0) t0 = globaltimer_ns();
-      __nanosleep(128);
-      if (globaltimer_ns() - t0 > g_budget_ns) {
-        *abort = 1;
-        atomicCAS(&g_record[0], 0u, code);
-        return false;
-      }
-    }
-  }
-}
-// wait_one for a converged warp.
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t code) {
-  if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
-  const bool ok = wait_one(bar, parity, abort, code);
-  return __all_sync(0xFFFFFFFFu, ok);
 }
 
 __device__ __forceinline__ uint32_t pair_bf16(float a, float b) {
@@ -642,22 +613,8 @@ int launch_form(const void* a, int64_t ld_a, const void* w, int64_t ld_w, BlockP
 
 }  // namespace
 
-int set_block_wait_budget_ns(uint64_t ns) { return (int)cudaMemcpyToSymbol(g_budget_ns, &ns, sizeof(ns)); }
-
-// The record of a timed-out wait of this kernel, and clears it.
-int take_block_timeout_record(uint32_t* record, cudaStream_t s) {
-  uint32_t host[4] = {0, 0, 0, 0};
-  cudaError_t e = cudaMemcpyFromSymbolAsync(host, g_record, sizeof(host), 0, cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  if (e != cudaSuccess) return (int)e;
-  *record = host[0];
-  if (host[0] != 0) {
-    const uint32_t zero[4] = {0, 0, 0, 0};
-    e = cudaMemcpyToSymbolAsync(g_record, zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  }
-  return (int)e;
-}
+int set_block_wait_budget_ns(uint64_t ns) { return set_budget_ns(ns); }
+int take_block_timeout_record(uint32_t* record, cudaStream_t s) { return take_record(record, s); }
 
 }  // namespace iflb200
 

@@ -123,6 +123,8 @@ int set_stack_wait_budget_ns(uint64_t ns);  // stack_persistent.cu
 int set_peer_wait_budget_ns(uint64_t ns);   // xgpu_ops.cu
 int set_block_wait_budget_ns(uint64_t ns);  // gemm_block.cu
 int take_block_timeout_record(uint32_t* record, cudaStream_t s);
+int set_attend_wait_budget_ns(uint64_t ns);  // cache_attn_tiles.cu
+int take_attend_timeout_record(uint32_t* record, cudaStream_t s);
 
 __device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t rank) {
   uint32_t r;
@@ -2194,6 +2196,7 @@ extern "C" int iflb200_set_wait_budget_us(int64_t microseconds) {
   if (e != cudaSuccess) return (int)e;
   int st = set_stack_wait_budget_ns(ns);
   if (st == 0) st = set_block_wait_budget_ns(ns);
+  if (st == 0) st = set_attend_wait_budget_ns(ns);
   return st != 0 ? st : set_peer_wait_budget_ns(ns);
 }
 
@@ -2220,9 +2223,10 @@ extern "C" int iflb200_gemm_take_timeout_record(uint32_t* record, void* stream) 
     e = cudaStreamSynchronize(s);
   }
   if (e != cudaSuccess) return (int)e;
-  uint32_t block = 0;
-  const int st = take_block_timeout_record(&block, s);
-  if (st == 0 && *record == 0) *record = block;
+  uint32_t block = 0, attend = 0;
+  int st = take_block_timeout_record(&block, s);
+  if (st == 0) st = take_attend_timeout_record(&attend, s);
+  if (st == 0 && *record == 0) *record = block ? block : attend;
   return st;
 }
 

@@ -98,3 +98,4 @@ def test_entry_points_reject_bad_arguments_before_any_launch():
     assert attend(dt=F32) == -4 and attend(q=None) == -1 and attend(lens=None) == -1 and attend(table=None) == -1
     assert attend(prefix=p, causal=0) == -1 and attend(cap=-1.0) == -1 and attend(cap=math.nan) == -1 and attend(scale=math.nan) == -1
     assert attend(ws=ctypes.c_void_p(4104), wb=8192) == -3 and attend(wb=-1) == -1
+    assert [lib.iflb200_cache_attention_set_form(f) for f in (0, 1, 2, 0, 3, -1)] == [0, 0, 0, 0, -1, -1]

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import block_ref as ref
+from instinctflash_b200 import _lib
 from instinctflash_b200.kernels import blocks, kv_cache, rope
 from util import u8
 
@@ -110,18 +111,26 @@ def test_append_of_strided_and_unaligned_rows():
 # ------------------------------------------------------------------ attention
 
 def check_attention(q, cache, table, lens, workspace=None, out=None, **kw):
+    """Every form of the operator against the reference; returns the result of the one that the rule takes."""
     out = torch.full_like(q, 7.5) if out is None else out
     before = out.clone()
-    kv_cache.cache_attention(q, cache, table, lens, out, workspace=workspace, **kw)
     names = dict(softcap="cap")
     want, written, tol = ref.attend(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, lens, eps=torch.finfo(q.dtype).eps,
                                     **{names.get(n, n): x for n, x in kw.items()})
-    got = out.cpu().double()
-    assert torch.equal(got[~written], before.cpu().double()[~written]), "rows that are not there were written"
-    got, want, tol = got[written], want[written], tol[written]
-    assert torch.equal(got.isnan(), want.isnan())
-    off = ((got - want).abs() - tol).nan_to_num(-1.0)
-    assert off.max() <= 0 if off.numel() else True, f"{float(off.max())} outside at {(off > 0).nonzero()[0].tolist()}"
+    want, tol = want[written], tol[written]
+    for form in (1, 2, 0):
+        out.copy_(before)
+        assert _lib.lib().iflb200_cache_attention_set_form(form) == 0
+        try:
+            kv_cache.cache_attention(q, cache, table, lens, out, workspace=workspace, **kw)
+        finally:
+            _lib.lib().iflb200_cache_attention_set_form(0)
+        got = out.cpu().double()
+        assert torch.equal(got[~written], before.cpu().double()[~written]), f"form {form}: rows that are not there were written"
+        got = got[written]
+        assert torch.equal(got.isnan(), want.isnan()), f"form {form}: NaN in other places"
+        off = ((got - want).abs() - tol).nan_to_num(-1.0)
+        assert off.numel() == 0 or off.max() <= 0, f"form {form}: {float(off.max())} outside at {(off > 0).nonzero()[0].tolist()}"
     return out
 
 
