@@ -11,24 +11,23 @@ namespace {
 __device__ uint32_t g_record[4];                   // role << 24 | barrier << 16 | low bits of a counter; 0: none
 __device__ uint64_t g_budget_ns = 2000000000ull;   // of one wait
 
-// Wait of one thread; false once the CTA gives up.
+// Wait of one thread; false once the CTA gives up.  (Short: a kernel has a dozen copies of it.)
 __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t code) {
-  if (mbar_try_wait(bar, parity)) return true;
   uint64_t t0 = 0;
-  uint32_t spins = 0;
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort) return false;
-    if (++spins > 2048) {
-      if (t0 == 0) t0 = globaltimer_ns();
-      __nanosleep(128);
-      if (globaltimer_ns() - t0 > g_budget_ns) {
+#pragma unroll 1
+  for (uint32_t spins = 1; !mbar_try_wait(bar, parity); ++spins) {
+    if (spins % 512 == 0) {
+      if (*abort) return false;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > g_budget_ns) {
         *abort = 1;
         atomicCAS(&g_record[0], 0u, code);
         return false;
       }
     }
   }
+  return true;
 }
 // The same for a converged warp.
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t code) {

@@ -15,9 +15,9 @@
 // and P would have, with 11 bits of P and no work on P but its rounding.  The MMA takes the values [key][D] as they lie
 // (transposed B operand).
 //
-//   warps 0..3, 4..7   softmax, one row a thread, and the output (D 256 has one row tile, whose S has two buffers instead)
-//   warps 8..11        codes from global memory through registers to f16 tiles, one tile ahead; a step's scales
-//   warp 12            MMA issuer, tensor memory
+//   warp 0               MMA issuer, tensor memory (the first warp: behind the others' work it issued an MMA every 300 clocks)
+//   warps 4..7, 8..11    softmax, one row a thread, and the output (D 256 has one row tile, whose S has two buffers instead)
+//   warps 12..19         codes from global memory through registers to f16 tiles, one tile ahead; a step's scales
 #include "bounded_wait.cuh"
 #include "cache_attn.cuh"
 
@@ -25,7 +25,8 @@ namespace iflb200 {
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kConvert = 8;  // converter warps
+constexpr int kThreads = 32 * (12 + kConvert);
 
 template <int D>
 struct Tiles {
@@ -41,7 +42,9 @@ struct Tiles {
   static constexpr int kQ = 128 * D * 2, kTile = BN * D * 2;  // bytes
   static constexpr int kMeta = NQ * kQ + 4 * kTile;
   static constexpr int kNan = kMeta + 4 * GR * 16;
-  static constexpr int kBar = kNan + D * 4 + 16;
+  static constexpr int kOff = kNan + D * 4 + 16;          // each converter warp's units of two steps: offset of the codes
+  static constexpr int kHole = kOff + kConvert * 2 * GR * 8;  // of four steps: whether a unit has no page
+  static constexpr int kBar = kHole + 16;
   static constexpr int kSmem = kBar + 24 * 8 + 16 + 1024;
 };
 
@@ -61,27 +64,23 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld_16c(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
-      "r"(r[30]), "r"(r[31])
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-template <int REGS>
-__device__ __forceinline__ void more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
-}
-template <int REGS>
-__device__ __forceinline__ void fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
-}
-
 // f16 operands, fp32 result; `mn_b`: the B operand lies with its N side contiguous
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool mn_b) {
   return (1u << 4) | (mn_b ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -137,7 +136,26 @@ __device__ __forceinline__ void load_row8(const T* q, float (&x)[8]) {
   }
 }
 
-template <int D, typename T>
+// Sixteen codes of key `key` without their NaNs, whose columns learn of the first key that has one.  (Out of line: it is
+// hardly ever run.)
+__device__ __noinline__ uint4 without_nans(uint4 codes, int* first_nan, int key) {
+  uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll 1
+  for (int e = 0; e < 16; ++e) {
+    const uint32_t at = e >> 2, shift = 8 * (e & 3);
+    const uint32_t word = at == 0 ? w[0] : (at == 1 ? w[1] : (at == 2 ? w[2] : w[3]));
+    if ((word >> shift & 0x7F) == 0x7F) {
+      atomicMin(first_nan + e, key);
+#pragma unroll
+      for (uint32_t z = 0; z < 4; ++z)
+        if (z == at) w[z] &= ~(0xFFu << shift);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// CAP, SLOPES: whether the scores are capped, and get a bias by distance; kernels of their own, for the size of the code.
+template <int D, typename T, bool CAP, bool SLOPES>
 __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const __grid_constant__ AttendArgs a, const int vec) {
   using L = Tiles<D>;
   constexpr int BN = L::BN, NQ = L::NQ, GR = L::GR;
@@ -174,9 +192,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(KFULL, i), 4);
+      mbar_init(bar(KFULL, i), kConvert);
       mbar_init(bar(KEMPTY, i), 1);
-      mbar_init(bar(VFULL, i), 4);
+      mbar_init(bar(VFULL, i), kConvert);
       mbar_init(bar(VEMPTY, i), 1);
       mbar_init(bar(SFULL, i), 1);
       mbar_init(bar(PFULL, i), 4);
@@ -190,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   }
   for (int i = threadIdx.x; i < D; i += kThreads) nan_at[i] = INT32_MAX;
   __syncwarp();
-  if (warp == 12) {
+  if (warp == 0) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
@@ -199,23 +217,23 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp < 4 * NQ) {
+  if (warp >= 4 && warp < 4 + 4 * NQ) {
     // ------------------------------------------------------------------ softmax and output
-    more_registers<184>();
-    const int slot = warp >> 2;
+    const int slot = (warp >> 2) - 1;
     const int r = slot * 128 + (warp & 3) * 32 + lane;
     const bool in = r < rows;
     const int tok = (row0 + (in ? r : 0)) / a.G, hq = h * a.G + (row0 + (in ? r : 0)) - tok * a.G;
     const int limit = in ? limit_of(row0 + r) : INT32_MAX;  // (a row that is not there needs no mask)
     const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
     const float pos = (float)(len - nq + tok);
-    const float slope = a.slopes ? a.slopes[hq] * kLog2e : 0.0f;
-    const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    const float slope = SLOPES ? a.slopes[hq] * kLog2e : 0.0f;
+    const float inv_cap = CAP ? 1.0f / a.cap : 0.0f;
     float factor;
     {
       // the row of q as f16, its largest element near 1
       const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_b + tok * a.q_t + hq * a.q_h;
       float top = 0.0f;
+#pragma unroll 1
       for (int i = 0; i < D / 8; ++i) {
         float x[8];
         if (vec) load_row8<T, true>(q + 8 * i, x);
@@ -228,6 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
       const float down = __uint_as_float((uint32_t)(254 - e2) << 23);
       factor = __uint_as_float((uint32_t)e2 << 23) * a.scale;
       const uint32_t at = q_at + slot * L::kQ + (r & 127) * 128;
+#pragma unroll 1
       for (int i = 0; i < D / 8; ++i) {
         float x[8];
         if (vec) load_row8<T, true>(q + 8 * i, x);
@@ -242,153 +261,195 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_at = tmem + lanes + kO + slot * D;
     float top_run = -INFINITY, l = 0.0f;
+    float drop = 1.0f;   // what O has yet to be multiplied by: a power of two
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
       const int buf = NQ == 2 ? slot : j & 1;
       const uint32_t phase = NQ == 2 ? j & 1u : (j >> 1) & 1u;
-      const uint32_t s_at = tmem + lanes + kS + buf * BN;
+      const uint32_t s_at = tmem + lanes + kS + buf * BN, p_at = tmem + lanes + L::kP + buf * L::kPStride;
       ok = wait_warp(bar(SFULL, buf), phase, abort_flag, (1u << 24) | (1u << 16) | (j & 0xFFFF));
       if (!ok) break;
       tc_fence_after();
-      uint32_t v[BN];
-#pragma unroll
-      for (int i = 0; i < BN / 32; ++i) tmem_ld_32x32b_x32(s_at + 32 * i, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * i));
-      const uint32_t m_at = meta + (j & 3) * GR * 16;
+      const uint32_t m_at = meta + (j & 3) * GR * 16;  // of each unit: ks, log2 vs, 1 / vs, 0 where there is no page
       const int key = key0 + j * BN;
-      // The product of the step before has to be complete ahead of a change of O, and every phase of its barrier is waited
-      // for in turn.  With two row tiles it was ahead of these scores; else it may run until the weights are ready.
-      bool waited = j == 0;
-      auto product_done = [&]() {
-        if (!waited) ok = wait_warp(bar(PV, slot), (j - 1) & 1u, abort_flag, (1u << 24) | (2u << 16) | (j & 0xFFFF));
-        waited = true;
-        tc_fence_after();
-      };
-      if (NQ == 2) product_done();
-      tmem_ld_wait();
-      float top = -INFINITY;
-      bool broken = false;
+      const bool edge = key + BN > least || *reinterpret_cast<volatile int*>(smem + L::kHole + (j & 3) * 4) != 0;
+      float4 m0, m1;
+      // Exponents of 32 columns (two units).  Everything here is a loop over 32 columns that is not unrolled: the parts of this
+      // kernel that run at the same time have to fit the instruction cache together.  With 128 columns unrolled an MMA was
+      // issued every 300 clocks (2048 tokens behind 6144, 32 heads: 746 us; @@ like this).
+      auto exponents = [&](int i, uint32_t (&v)[32]) {
+        tmem_ld_32x32b_x32(s_at + 32 * i, v);
+        m0 = lds_f4(m_at + 32 * i);
+        m1 = lds_f4(m_at + 32 * i + 16);
+        const float f0 = factor * m0.x * (CAP ? 1.0f : kLog2e), f1 = factor * m1.x * (CAP ? 1.0f : kLog2e);
+        const float base = top_run == -INFINITY ? 0.0f : top_run, c0 = m0.y - base, c1 = m1.y - base;
+        tmem_ld_wait();
+        if (CAP) {
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {
-        const float4 m = lds_f4(m_at + 16 * g);  // ks, log2 vs, 1 / vs, 0 where there is no page
-        broken |= m.w == 0.0f;
-        const float f = factor * m.x;
-        if (a.cap > 0.0f) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            v[16 * g + e] = __float_as_uint(fmaf(soft_cap(__uint_as_float(v[16 * g + e]) * f, a.cap, inv_cap), kLog2e, m.y));
+          for (int e = 0; e < 32; ++e)
+            v[e] = __float_as_uint(fmaf(soft_cap(__uint_as_float(v[e]) * (e < 16 ? f0 : f1), a.cap, inv_cap), kLog2e, e < 16 ? c0 : c1));
         } else {
-          const uint64_t f2 = pack2(f * kLog2e, f * kLog2e), y2 = pack2(m.y, m.y);
+          const uint64_t f[2] = {pack2(f0, f0), pack2(f1, f1)}, c[2] = {pack2(c0, c0), pack2(c1, c1)};
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
+          for (int e = 0; e < 32; e += 2) {
             float p0, p1;
-            unpack2(fma2(pack2(__uint_as_float(v[16 * g + e]), __uint_as_float(v[16 * g + e + 1])), f2, y2), p0, p1);
-            v[16 * g + e] = __float_as_uint(p0);
-            v[16 * g + e + 1] = __float_as_uint(p1);
+            unpack2(fma2(pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f[e >> 4], c[e >> 4]), p0, p1);
+            v[e] = __float_as_uint(p0);
+            v[e + 1] = __float_as_uint(p1);
           }
         }
-      }
-      if (a.slopes) {
-        const float from = pos - (float)key;
+        if (SLOPES) {
+          const float from = pos - (float)(key + 32 * i);
 #pragma unroll
-        for (int e = 0; e < BN; ++e) v[e] = __float_as_uint(fmaf(-slope, fabsf(from - (float)e), __uint_as_float(v[e])));
-      }
-      if (key + BN > least || broken) {
-        const int n = limit - key;
-#pragma unroll
-        for (int g = 0; g < GR; ++g) {
-          const bool gone = lds_f4(m_at + 16 * g).w == 0.0f;
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (16 * g + e >= n || gone) v[16 * g + e] = 0xFF800000u;
+          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fmaf(-slope, fabsf(from - (float)e), __uint_as_float(v[e])));
         }
-      }
+        if (edge) {
+          const int n = limit - key - 32 * i, n0 = m0.w == 0.0f ? 0 : n, n1 = m1.w == 0.0f ? 0 : n;
 #pragma unroll
-      for (int e = 0; e < BN; e += 2) top = max3(top, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-      if (__any_sync(0xFFFFFFFFu, top > top_run + kLazy)) {
-        const float now = fmaxf(top_run, top);
-        const float f = top_run == -INFINITY ? 0.0f : ex2_approx_ftz(top_run - now);
-        top_run = now;
-        l *= f;
-        if (j > 0) {
-          if (NQ == 1) product_done();
+          for (int e = 0; e < 32; ++e)
+            if (e >= (e < 16 ? n0 : n1)) v[e] = 0xFF800000u;
+        }
+        float high = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) high = max3(high, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+        return high;
+      };
+      // O may change once the product of the step before is complete, and every phase of its barrier is waited for in turn.
+      auto settle = [&]() {
+        if (j > 0) ok = wait_warp(bar(PV, slot), (j - 1) & 1u, abort_flag, (1u << 24) | (2u << 16) | (j & 0xFFFF));
+        tc_fence_after();
+        if (ok && __any_sync(0xFFFFFFFFu, drop != 1.0f)) {
+          if (j > 0) {
 #pragma unroll 1
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(o_at + 32 * i, o);
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t o[16];
+              tmem_ld_16c(o_at + 16 * i, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * drop);
+              tmem_st_16(o_at + 16 * i, o);
+            }
+            tmem_st_wait();
+          }
+          drop = 1.0f;
+        }
+      };
+      // A row without a maximum yet gets that of these scores.
+      if (__any_sync(0xFFFFFFFFu, top_run == -INFINITY)) {
+        float first = -INFINITY;
+        const bool none = top_run == -INFINITY;
+#pragma unroll 1
+        for (int i = 0; i < BN / 32; ++i) {
+          uint32_t v[32];
+          first = fmaxf(first, exponents(i, v));
+        }
+        if (none) top_run = first;
+      }
+      // The weights, relative to the maximum of the steps before: f16 has room for 2^15 of it.
+      float high = -INFINITY;
+#pragma unroll 1
+      for (int i = 0; i < BN / 32; ++i) {
+        uint32_t v[32];
+        const float now = exponents(i, v);
+        high = fmaxf(high, now);
+        if (__any_sync(0xFFFFFFFFu, now > 15.0f)) {
+          // more than that: all there is moves down, the weights of this step that are stored already too
+          const float by = now > 15.0f ? ceilf(now) : 0.0f, f = ex2_approx_ftz(-by);
+          const uint32_t f2 = pack_half2(f, f);
+          if (by > 0.0f) top_run += by;
+          high = by > 0.0f ? 0.0f : high;
+          l *= f;
+          drop *= f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) - by);
+          tmem_st_wait();
+#pragma unroll 1
+          for (int z = 0; z < i; ++z) {
+            uint32_t w[16];
+            tmem_ld_16c(p_at + 16 * z, w);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st_32(o_at + 32 * i, o);
+            for (int e = 0; e < 16; ++e) {
+              const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&w[e]), *reinterpret_cast<const __half2*>(&f2));
+              w[e] = *reinterpret_cast<const uint32_t*>(&x);
+            }
+            tmem_st_16(p_at + 16 * z, w);
           }
-          tmem_st_wait();
         }
-      }
-      const float m = top_run == -INFINITY ? 0.0f : top_run;
+        uint64_t t[2] = {0, 0};
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float p0 = ex2_approx_ftz(__uint_as_float(v[16 * g + e]) - m), p1 = ex2_approx_ftz(__uint_as_float(v[16 * g + e + 1]) - m);
-          s += p0 + p1;
-          v[8 * g + e / 2] = pack_half2(p0, p1);
+        for (int e = 0; e < 32; e += 2) {
+          const float p0 = ex2_approx_ftz(__uint_as_float(v[e])), p1 = ex2_approx_ftz(__uint_as_float(v[e + 1]));
+          t[e >> 4] = add2(t[e >> 4], pack2(p0, p1));
+          v[e / 2] = pack_half2(p0, p1);
         }
-        l = fmaf(s, lds_f4(m_at + 16 * g).z, l);
+        float t0, t1;
+        unpack2(t[0], t0, t1);
+        l = fmaf(t0 + t1, m0.z, l);
+        unpack2(t[1], t0, t1);
+        l = fmaf(t0 + t1, m1.z, l);
+        // (over scores that have been read, where the weights have no columns of their own)
+        tmem_st_16(p_at + 16 * i, *reinterpret_cast<uint32_t(*)[16]>(v));
       }
-      product_done();
+      settle();
       if (!ok) break;
-#pragma unroll
-      for (int i = 0; i < BN / 64; ++i) tmem_st_32(tmem + lanes + L::kP + buf * L::kPStride + 32 * i, v + 32 * i);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(PFULL, buf));
+      // the maximum moves when a score has passed it by more than kLazy, by a whole power of two; O follows at the next step
+      if (__any_sync(0xFFFFFFFFu, high > kLazy)) {
+        const float by = high > kLazy ? ceilf(high) : 0.0f, f = ex2_approx_ftz(-by);
+        if (by > 0.0f) top_run += by;
+        l *= f;
+        drop = f;
+      }
     }
     if (ok && steps > 0) ok = wait_warp(bar(PV, slot), (steps - 1) & 1u, abort_flag, (1u << 24) | (3u << 16));
     tc_fence_after();
     const int ticket = b * a.H * a.row_tiles + y;
     const bool any_nan = *nan_any != 0;
-    const float inv = chunks > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+    const float inv = drop * (chunks > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l));  // (the last move of the maximum is still to be made)
     T* out = reinterpret_cast<T*>(a.out) + b * a.o_b + tok * a.o_t + hq * a.o_h;
     const int64_t at = ((int64_t)ticket * a.splits + split) * L::ROWS + r;
     float* part = a.partial + at * D;
 #pragma unroll 1
-    for (int i = 0; i < D / 32; ++i) {
-      uint32_t o[32];
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t o[16];
       if (steps > 0) {
-        tmem_ld_32x32b_x32(o_at + 32 * i, o);
+        tmem_ld_16c(o_at + 16 * i, o);
         tmem_ld_wait();
       } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0;
+        for (int e = 0; e < 16; ++e) o[e] = 0;
       }
       if (in && ok) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < 16; ++e) {
           float x = __uint_as_float(o[e]) * inv;
-          if (any_nan && nan_at[32 * i + e] < limit) x = __uint_as_float(0x7FC00000u);
+          if (any_nan && nan_at[16 * i + e] < limit) x = __uint_as_float(0x7FC00000u);
           o[e] = __float_as_uint(x);
         }
         if (chunks > 1) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(part + 32 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<uint4*>(part + 16 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         } else if (vec) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
+          for (int e = 0; e < 16; e += 8) {
             uint4 u;
             uint32_t* w = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
             for (int z = 0; z < 4; ++z) w[z] = pack_out<T>(__uint_as_float(o[e + 2 * z]), __uint_as_float(o[e + 2 * z + 1]));
-            *reinterpret_cast<uint4*>(out + 32 * i + e) = u;
+            *reinterpret_cast<uint4*>(out + 16 * i + e) = u;
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
+          for (int e = 0; e < 16; e += 2) {
             const uint32_t w = pack_out<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
             const T* two = reinterpret_cast<const T*>(&w);
-            out[32 * i + e] = two[0];
-            out[32 * i + e + 1] = two[1];
+            out[16 * i + e] = two[0];
+            out[16 * i + e + 1] = two[1];
           }
         }
       }
@@ -399,15 +460,15 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
       // the last CTA of the chunks adds them up, in their order
       __threadfence();
       named_bar_sync(1, 128 * NQ);
-      if (threadIdx.x == 0) *last_one = atomicAdd(a.tickets + ticket, 1u) == (uint32_t)chunks - 1;
+      if (threadIdx.x == 128) *last_one = atomicAdd(a.tickets + ticket, 1u) == (uint32_t)chunks - 1;
       named_bar_sync(1, 128 * NQ);
       if (*last_one) {
         __threadfence();
-        if (threadIdx.x == 0) a.tickets[ticket] = 0;
+        if (threadIdx.x == 128) a.tickets[ticket] = 0;
         const int64_t from = (int64_t)ticket * a.splits * L::ROWS;
         const float2* ml = reinterpret_cast<const float2*>(a.partial + a.partial_ml) + from;
         const float* po = a.partial + from * D;
-        for (int i = threadIdx.x; i < rows * (D / 4); i += 128 * NQ) {
+        for (int i = threadIdx.x - 128; i < rows * (D / 4); i += 128 * NQ) {
           const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4;
           float mm = -INFINITY;
           for (int s = 0; s < chunks; ++s) mm = fmaxf(mm, __ldcg(ml + s * L::ROWS + rr).x);
@@ -439,13 +500,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
         }
       }
     }
-  } else if (warp < 8) {
-    fewer_registers<40>();
-  } else if (warp < 12) {
+  } else if (warp >= 12) {
     // ------------------------------------------------------------------ codes to f16 tiles
-    fewer_registers<96>();
-    constexpr int CH = D / 16, UN = BN * CH / 128, TPI = 128 / CH;  // chunks of a key, chunks a thread, keys apart
-    const int tid = threadIdx.x - 256, chunk = tid % CH, first = tid / CH;
+    constexpr int CH = D / 16, UN = BN * CH / (32 * kConvert), TPI = 32 * kConvert / CH;  // chunks of a key, chunks a thread, keys apart
+    // Eight lanes store four pieces of one key and four of the next, which the swizzle puts on other banks.
+    const int tid = threadIdx.x - 384, chunk = (tid & 3) | ((tid >> 3) & (CH / 4 - 1)) << 2, first = (tid >> 2 & 1) | (tid >> 3) / (CH / 4) << 1;
     const int32_t* table = a.table + b * a.ld_table;
     auto raw_page = [&](int step) {  // of this lane's unit of the step
       const int key = key0 + step * BN + 16 * lane;
@@ -453,22 +512,27 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     };
     int page = raw_page(0), page_next = raw_page(1);
     float ks = 0.0f, vs = 0.0f;
-    int64_t off = -1;
-    auto look_up = [&](int step) {  // where this lane's unit lies, and its scales
-      const bool there = page >= 0 && page < a.pages;
+    bool there = false;
+    // Where the units of a step lie, through shared memory to the warp's lanes; -1: no page.
+    int64_t* offs = reinterpret_cast<int64_t*>(smem + L::kOff) + (warp - 12) * 2 * GR;
+    auto look_up = [&](int step) {
+      there = page >= 0 && page < a.pages;
       const int key = key0 + step * BN + 16 * lane;
-      off = there ? (((int64_t)page * a.H + h) * a.P + key % a.P) * D : -1;
+      if (lane < GR) offs[(step & 1) * GR + lane] = there ? (((int64_t)page * a.H + h) * a.P + key % a.P) * D : -1;
       ks = there ? __ldg(a.ks + (int64_t)page * a.H + h) : 0.0f;
       vs = there ? __ldg(a.vs + (int64_t)page * a.H + h) : 0.0f;
+      __syncwarp();
     };
     uint4 kr[UN], vr[UN];
+    // (what is not there is read at the cache's beginning and made zero: no branch around a load)
     auto load = [&](const uint8_t* codes, int step, uint4 (&r)[UN]) {
 #pragma unroll
       for (int i = 0; i < UN; ++i) {
         const int t = i * TPI + first;
-        const int64_t o = __shfl_sync(0xFFFFFFFFu, off, t >> 4);
-        r[i] = make_uint4(0, 0, 0, 0);
-        if (o >= 0 && key0 + step * BN + t < key1) r[i] = __ldg(reinterpret_cast<const uint4*>(codes + o + (t & 15) * D + chunk * 16));
+        const int64_t o = offs[(step & 1) * GR + (t >> 4)];
+        const bool in = o >= 0 && key0 + step * BN + t < key1;
+        r[i] = __ldg(reinterpret_cast<const uint4*>(codes + (in ? o + (t & 15) * D : 0) + chunk * 16));
+        if (!in) r[i] = make_uint4(0, 0, 0, 0);
       }
     };
     auto write = [&](uint32_t tile, const uint4 (&r)[UN]) {
@@ -476,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
       for (int i = 0; i < UN; ++i) {
         const int t = i * TPI + first;
         const uint32_t at = tile + (chunk >> 2) * BN * 128 + t * 128;
-        const uint32_t c0 = (chunk & 3) * 2, odd = chunk >> 2 & 1;  // (halves of a key store in turn: no bank twice)
+        const uint32_t c0 = (chunk & 3) * 2;
         const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
         uint32_t f[8];
 #pragma unroll
@@ -484,45 +548,45 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
           f[2 * e] = e4m3x2_f16x2(w[e]);
           f[2 * e + 1] = e4m3x2_f16x2(w[e] >> 16);
         }
-        const uint32_t lo = at + ((c0 ^ (t & 7)) << 4), hi = at + (((c0 + 1) ^ (t & 7)) << 4);
-        if (odd) {
-          sts128(hi, f[4], f[5], f[6], f[7]);
-          sts128(lo, f[0], f[1], f[2], f[3]);
-        } else {
-          sts128(lo, f[0], f[1], f[2], f[3]);
-          sts128(hi, f[4], f[5], f[6], f[7]);
-        }
+        sts128(at + ((c0 ^ (t & 7)) << 4), f[0], f[1], f[2], f[3]);
+        sts128(at + (((c0 + 1) ^ (t & 7)) << 4), f[4], f[5], f[6], f[7]);
       }
       fence_proxy_async_smem();
       __syncwarp();
     };
     bool ok = true;
-    if (steps > 0) {
-      look_up(0);
-      load(a.k, 0, kr);
-      load(a.v, 0, vr);
-    }
-    for (int j = 0; j < steps; ++j) {
+    uint32_t zero_units = 0;
+    for (int j = -1; j < steps; ++j) {  // (-1: loads only)
+      if (j >= 0) {
       const int s = j & 1;
       const uint32_t phase = (j >> 1) & 1u;
       // pages with a value scale of zero: their weights count, their values are zeros
       const float vs_now = vs;
-      const uint32_t zero_units = __ballot_sync(0xFFFFFFFFu, vs_now == 0.0f);
-      if (warp == 8 && lane < GR) {
+      zero_units = __ballot_sync(0xFFFFFFFFu, vs_now == 0.0f);
+      const uint32_t holes = __ballot_sync(0xFFFFFFFFu, lane < GR && !there);
+      if (warp == 12 && lane == 0) *reinterpret_cast<int*>(smem + L::kHole + (j & 3) * 4) = holes != 0;
+      if (warp == 12 && lane < GR) {
         const float lv = vs_now == 0.0f ? 0.0f : log2_approx(vs_now);
         *reinterpret_cast<float4*>(smem + L::kMeta + (j & 3) * GR * 16 + lane * 16) =
-            make_float4(ks, lv, vs_now == 0.0f ? 1.0f : 1.0f / vs_now, off >= 0 ? 1.0f : 0.0f);
+            make_float4(ks, lv, vs_now == 0.0f ? 1.0f : 1.0f / vs_now, there ? 1.0f : 0.0f);
       }
       ok = wait_warp(bar(KEMPTY, s), phase ^ 1u, abort_flag, (2u << 24) | (4u << 16) | (j & 0xFFFF));
       if (!ok) break;
       write(k_at + s * L::kTile, kr);
       if (lane == 0) mbar_arrive(bar(KFULL, s));
-      page = page_next;
+      // (zero_units: of this step, the look-up below is the next one's)
+      }
       if (j + 1 < steps) {
-        page_next = raw_page(j + 2);
+        if (j >= 0) {
+          page = page_next;
+          page_next = raw_page(j + 2);
+        }
         look_up(j + 1);
         load(a.k, j + 1, kr);
       }
+      if (j >= 0) {
+      const int s = j & 1;
+      const uint32_t phase = (j >> 1) & 1u;
       // NaN codes become zeros, and where the first one of a column is goes to the output's warps
 #pragma unroll
       for (int i = 0; i < UN; ++i) {
@@ -533,25 +597,20 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
                              __vcmpeq4(w[2] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) | __vcmpeq4(w[3] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
         if (hit) {
           *nan_any = 1;
-          for (int e = 0; e < 16; ++e) {
-            if ((w[e >> 2] >> (8 * (e & 3)) & 0x7F) == 0x7F) {
-              atomicMin(nan_at + chunk * 16 + e, key0 + j * BN + t);
-              w[e >> 2] &= ~(0xFFu << (8 * (e & 3)));
-            }
-          }
+          vr[i] = without_nans(vr[i], nan_at + chunk * 16, key0 + j * BN + t);
         }
       }
       ok = wait_warp(bar(VEMPTY, s), phase ^ 1u, abort_flag, (2u << 24) | (5u << 16) | (j & 0xFFFF));
       if (!ok) break;
       write(v_at + s * L::kTile, vr);
       if (lane == 0) mbar_arrive(bar(VFULL, s));
+      }
       if (j + 1 < steps) load(a.v, j + 1, vr);
     }
     grid_launch_dependents();
-  } else {
-    fewer_registers<40>();
+  } else if (warp < 4) {
     // ------------------------------------------------------------------ MMA issuer
-    if (warp == 12 && elect_one() && steps > 0) {
+    if (warp == 0 && elect_one() && steps > 0) {
       constexpr uint32_t id_s = idesc_f16(128, BN, false), id_o = idesc_f16(128, D, true);
       auto scores = [&](int j, int slot, int buf) {
         const uint64_t dq = make_kmajor_sw128_desc(q_at + slot * L::kQ), dk = make_kmajor_sw128_desc(k_at + (j & 1) * L::kTile);
@@ -568,82 +627,66 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
           mma_f16_ts(tmem + kO + slot * D, tmem + L::kP + buf * L::kPStride + 8 * k, dv + k * 2048 / 16, id_o, j > 0 || k > 0);
         mma_commit(bar(PV, slot));
       };
+      // Scores are AHEAD steps ahead of products: one with two row tiles in turn, two with two buffers.
+      constexpr int AHEAD = NQ == 2 ? 1 : 2;
       bool ok = wait_one(bar(QFULL, 0), 0, abort_flag, (3u << 24) | (6u << 16));
-      auto keys = [&](int j) {
-        ok = ok && wait_one(bar(KFULL, j & 1), (j >> 1) & 1u, abort_flag, (3u << 24) | (7u << 16) | (j & 0xFFFF));
-        tc_fence_after();
-      };
-      keys(0);
-      if (ok) {
-        scores(0, 0, 0);
-        if (NQ == 2) scores(0, 1, 1);
-        if (steps > 2) mma_commit(bar(KEMPTY, 0));  // (here and below: only where a later tile waits for it)
-      }
-      if (NQ == 1 && steps > 1) {
-        keys(1);
-        if (ok) {
-          scores(1, 0, 1);
-          if (steps > 3) mma_commit(bar(KEMPTY, 1));
-        }
-      }
-      for (int j = 0; ok && j < steps; ++j) {
-        ok = wait_one(bar(VFULL, j & 1), (j >> 1) & 1u, abort_flag, (3u << 24) | (8u << 16) | (j & 0xFFFF));
-        if (NQ == 2) {
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            ok = ok && wait_one(bar(PFULL, s), j & 1u, abort_flag, (3u << 24) | (9u << 16) | (j & 0xFFFF));
+#pragma unroll 1
+      for (int j = -AHEAD; ok && j < steps; ++j) {
+        const int n = j + AHEAD;  // whose scores are next
+#pragma unroll 1
+        for (int slot = 0; ok && slot < NQ; ++slot) {
+          const int buf = NQ == 2 ? slot : j & 1;
+          if (j >= 0) {
+            if (slot == 0) ok = wait_one(bar(VFULL, j & 1), (j >> 1) & 1u, abort_flag, (3u << 24) | (8u << 16) | (j & 0xFFFF));
+            ok = ok && wait_one(bar(PFULL, buf), NQ == 2 ? j & 1u : (j >> 1) & 1u, abort_flag, (3u << 24) | (9u << 16) | (j & 0xFFFF));
             if (!ok) break;
             tc_fence_after();
-            product(j, s, s);
-            if (j + 1 < steps) {
-              if (s == 0) keys(j + 1);
-              if (L::kOver) ok = ok && wait_one(bar(PV, s), j & 1u, abort_flag, (3u << 24) | (10u << 16) | (j & 0xFFFF));
-              if (ok) scores(j + 1, s, s);
-            }
+            product(j, slot, buf);
           }
-          if (!ok) break;
-          if (j + 2 < steps) mma_commit(bar(VEMPTY, j & 1));
-          if (j + 3 < steps) mma_commit(bar(KEMPTY, (j + 1) & 1));
-        } else {
-          ok = ok && wait_one(bar(PFULL, j & 1), (j >> 1) & 1u, abort_flag, (3u << 24) | (9u << 16) | (j & 0xFFFF));
-          if (!ok) break;
-          tc_fence_after();
-          product(j, 0, j & 1);
-          if (j + 2 < steps) mma_commit(bar(VEMPTY, j & 1));
-          if (j + 2 < steps) {
-            keys(j + 2);
+          if (n < steps) {
+            if (slot == 0) ok = wait_one(bar(KFULL, n & 1), (n >> 1) & 1u, abort_flag, (3u << 24) | (7u << 16) | (n & 0xFFFF));
+            if (L::kOver && j >= 0) ok = ok && wait_one(bar(PV, slot), j & 1u, abort_flag, (3u << 24) | (10u << 16) | (j & 0xFFFF));
             if (!ok) break;
-            scores(j + 2, 0, j & 1);
-            if (j + 4 < steps) mma_commit(bar(KEMPTY, j & 1));
+            tc_fence_after();
+            scores(n, slot, buf);
           }
         }
+        // given back only where a later step waits for it
+        if (ok && j >= 0 && j + 2 < steps) mma_commit(bar(VEMPTY, j & 1));
+        if (ok && n + 2 < steps) mma_commit(bar(KEMPTY, n & 1));
       }
     }
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
 
-template <int D, typename T>
+template <int D, typename T, bool CAP, bool SLOPES>
 int launch_tiles(const AttendArgs& a, int vec, cudaStream_t s) {
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return IFLB200_ERR_DEVICE;
   if (!attr_set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(cache_attend_tiles_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tiles<D>::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(cache_attend_tiles_kernel<D, T, CAP, SLOPES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tiles<D>::kSmem);
     if (e != cudaSuccess) return (int)e;
     attr_set[dev] = true;
   }
   const dim3 grid((unsigned)a.splits, (unsigned)(a.H * a.row_tiles), (unsigned)a.B);
-  const cudaError_t e = launch_dep(cache_attend_tiles_kernel<D, T>, grid, dim3(kThreads), Tiles<D>::kSmem, s, 1,
+  const cudaError_t e = launch_dep(cache_attend_tiles_kernel<D, T, CAP, SLOPES>, grid, dim3(kThreads), Tiles<D>::kSmem, s, 1,
                                    dependent_launch_for((int64_t)a.B * a.T), a, vec);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+template <int D, typename T>
+int launch_tiles(const AttendArgs& a, int vec, cudaStream_t s) {
+  if (a.cap > 0.0f) return a.slopes ? launch_tiles<D, T, true, true>(a, vec, s) : launch_tiles<D, T, true, false>(a, vec, s);
+  return a.slopes ? launch_tiles<D, T, false, true>(a, vec, s) : launch_tiles<D, T, false, false>(a, vec, s);
 }
 
 }  // namespace
