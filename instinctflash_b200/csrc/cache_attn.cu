@@ -37,46 +37,129 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-// 1.0 in each half of x that is a NaN (all bits below the sign set: what a NaN code converts to), else 0.
-__device__ __forceinline__ uint32_t nan_halves(uint32_t x) {
-  return ((x & 0x7FFF) > 0x7C00 ? 0x3C00u : 0u) | ((x & 0x7FFF0000u) > 0x7C000000u ? 0x3C000000u : 0u);
-}
-__device__ __forceinline__ uint32_t without_nan(uint32_t x) {
-  return ((x & 0x7FFF) > 0x7C00 ? 0u : x & 0xFFFF) | ((x & 0x7FFF0000u) > 0x7C000000u ? 0u : x & 0xFFFF0000u);
-}
-
 // ---------------------------------------------------------------------------------------------
 // Few rows (query token x head of a group): bound by the cache's bytes.
 //
 // Keys on the MMA's M side, 8 rows on its N side.  Every warp walks key tiles of its own with a softmax state of its
-// own, loads (cp.async, three tiles ahead, 16-byte pieces swizzled for ldmatrix) and all: no barrier until the end.
+// own, loads (cp.async, two tiles ahead, 16-byte pieces swizzled for ldmatrix) and all: no barrier until the end.
 // Codes become f16 in registers, which is exact; q is f16 too, its row brought near 1 by a power of two (a bf16 row keeps
 // all its bits down to 2^-14 of its largest element); weights are f16 relative to the row's running maximum.  All sums
-// and the softmax state are fp32.  The two scales of a page are uniform over 16 keys: ks goes into the factor of the
-// scores, vs / (the scale that the output is kept in) into the weights ahead of their rounding.
+// and the softmax state are fp32.
+//
+// The scales of a page are uniform over 16 keys: ks is part of the scores' factor, vs part of the exponent, as in
+// cache_attn_tiles.cu: weights 2^(y - M) with y = x + log2 vs, l = sum 2^(y - M) / vs, output = (sum of weights times
+// codes) / l.  Sixteen tiles' pages and scales are looked up at a time, one unit of sixteen keys a lane.
+//
+// The code is kept short (loops over stages are not unrolled, what is rare is out of the way): a step of few rows is as much
+// instruction fetch as memory.  @@
 // ---------------------------------------------------------------------------------------------
-template <int D, int NT, typename T>
-__global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __grid_constant__ AttendArgs a) {
+
+// NaN codes of a tile's values: the first key that has one, by column, and zeros in their place.
+__device__ __noinline__ void take_nans(uint32_t vt, int bytes, int D, int key, int lane, int* first_nan) {
+#pragma unroll 1
+  for (int i = lane; i < bytes / 4; i += 32) {
+    uint32_t w;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(vt + 4 * i));
+    if (__vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu) == 0) continue;
+    const int row = 4 * i / D, at = 4 * i % D, chunk = at >> 4;
+    const int d = (D == 64 ? chunk ^ (row >> 1 & 3) : chunk ^ (row & 7)) * 16 + (at & 15);
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) {
+      if ((w >> (8 * e) & 0x7F) == 0x7F) {
+        atomicMin(first_nan + d + e, key + row);
+        w &= ~(0xFFu << (8 * e));
+      }
+    }
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(vt + 4 * i), "r"(w) : "memory");
+  }
+  __syncwarp();
+}
+
+template <int D, int NT, typename T, bool CAP>
+__global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __grid_constant__ AttendArgs a, const int vec) {
   constexpr int ROWS = 8 * NT, CH = D / 16, KB = kTile * D;  // 16-byte chunks of a key, bytes of a tile of K or V
   constexpr int LPR = CH, RPI = 32 / LPR;                    // lanes a key, keys an instruction of cp.async
+  constexpr int STEP = kWarps * kTile;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float m_of[kWarps][ROWS], l_of[kWarps][ROWS];
+  __shared__ int first_nan[D];
+  __shared__ int limits[ROWS];
+  __shared__ float4 unit[kWarps][kStages][2];  // of a stage's units: ks, log2 vs, 1 / vs, weight in the product (-1: no page)
   __shared__ uint32_t last_one;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, y = blockIdx.y, b = blockIdx.z;
   const int h = y / a.row_tiles, row0 = (y - h * a.row_tiles) * ROWS;
+  for (int i = threadIdx.x; i < D; i += 32 * kWarps) first_nan[i] = INT32_MAX;
   grid_dependency_wait();
-  const int len = min(max(a.lens[b], 0), (int)min((int64_t)a.max_pages * a.P, (int64_t)INT32_MAX));
+  const int room = a.max_pages * a.P;   // (at most 2^30)
+  const int key0 = split * a.chunk, first = key0 + warp * kTile;
+  const int32_t* table = a.table + b * a.ld_table;
+  // this lane's unit of the sixteen tiles from `tile` on
+  auto raw_page = [&](int tile) {
+    const int key = first + (tile + (lane >> 1)) * STEP + 16 * (lane & 1);
+    return key < room ? __ldg(table + key / a.P) : -1;
+  };
+  int page = raw_page(0), page_next = -1;
+  const int len = min(max(a.lens[b], 0), room);
   const int nq = a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
+  const int prefix = a.prefix ? a.prefix[b] : 0;
   const int rows = min(ROWS, nq * a.G - row0);
   if (rows <= 0) return;
-  const int prefix = a.prefix ? a.prefix[b] : 0;
   auto limit_of = [&](int r) { return a.causal ? min(len, max(len - nq + r / a.G + 1, prefix)) : len; };
   // limits grow with the row: the last row's is the largest, the first one's the smallest
   const int most = max(0, limit_of(row0 + rows - 1)), least = limit_of(row0);
   const int chunks = max(1, (most + a.chunk - 1) / a.chunk);
   if (split >= chunks) return;
-  const int key0 = split * a.chunk, key1 = min(most, key0 + a.chunk);
+  const int key1 = min(most, key0 + a.chunk);
+  if (threadIdx.x < ROWS) limits[threadIdx.x] = (int)threadIdx.x < rows ? limit_of(row0 + threadIdx.x) : 0;
+  __syncthreads();
+
+  const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * KB;
+  const int64_t head_bytes = (int64_t)a.P * D;
+  float ks = 0.0f, vs = 0.0f;
+  int in_page = 0;  // of this lane's unit: its first key in the page
+  auto look_up = [&](int tile) {
+    const int key = first + (tile + (lane >> 1)) * STEP + 16 * (lane & 1);
+    if (page < 0 || page >= a.pages || key >= key1) page = -1;
+    in_page = key % a.P;
+    ks = page >= 0 ? __ldg(a.ks + (int64_t)page * a.H + h) : 0.0f;
+    vs = page >= 0 ? __ldg(a.vs + (int64_t)page * a.H + h) : 0.0f;
+  };
+  // Tile `tile` into its stage; its units are lanes 2 (tile % 16) and the next.  What is not there becomes zeros.
+  const int load_row = lane / LPR, load_chunk = lane % LPR;
+  auto fetch = [&](int tile, int stage) {
+    const int key = first + tile * STEP;
+    if (key < key1) {
+      const int src = 2 * (tile & 15);
+      if (src == 0) {
+        if (tile > 0) page = page_next;
+        look_up(tile);
+      } else if (src == 16) {
+        page_next = raw_page(tile + 8);
+      }
+      if ((lane >> 1) == (tile & 15)) {
+        // (a value scale of zero: the weights count, their product is nothing)
+        const bool nil = vs == 0.0f;
+        unit[warp][stage][lane & 1] = make_float4(ks, nil ? 0.0f : log2_approx(vs), nil ? 1.0f : 1.0f / vs, page < 0 ? -1.0f : (nil ? 0.0f : 1.0f));
+      }
+      const int p0 = __shfl_sync(0xFFFFFFFFu, page, src), p1 = __shfl_sync(0xFFFFFFFFu, page, src + 1);
+      const int i0 = __shfl_sync(0xFFFFFFFFu, in_page, src), i1 = __shfl_sync(0xFFFFFFFFu, in_page, src + 1);
+      const int64_t o0 = ((int64_t)max(p0, 0) * a.H + h) * head_bytes + i0 * D, o1 = ((int64_t)max(p1, 0) * a.H + h) * head_bytes + i1 * D;
+      const uint32_t dst = ring + stage * 2 * KB;
+#pragma unroll
+      for (int i = 0; i < kTile / RPI; ++i) {
+        const int row = i * RPI + load_row;
+        const bool in = key + row < key1 && (i < kTile / RPI / 2 ? p0 : p1) >= 0;
+        const int64_t off = in ? (i < kTile / RPI / 2 ? o0 : o1) + (row & 15) * D + load_chunk * 16 : 0;
+        const uint32_t at = dst + row * D + (D == 64 ? load_chunk ^ (row >> 1 & 3) : load_chunk ^ (row & 7)) * 16;
+        cp_async_16(at, a.k + off, in ? 16 : 0);
+        cp_async_16(at + KB, a.v + off, in ? 16 : 0);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int s = 0; s < kStages - 1; ++s) fetch(s, s);
 
   // this thread's columns of the scores: rows 8 n + 2 c + e
   float factor[NT][2], slope[NT][2], pos[NT][2];
@@ -87,15 +170,29 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
     const int r = 8 * n + g;
     const bool in = r < rows;
     const int t = (row0 + (in ? r : 0)) / a.G, hq = h * a.G + (row0 + (in ? r : 0)) - t * a.G;
-    const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_b + t * a.q_t + hq * a.q_h;
+    const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_b + t * a.q_t + hq * a.q_h + 4 * c;
+    uint2 x[CH];
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) x[i] = *reinterpret_cast<const uint2*>(q + 16 * i);
+    } else {
+      const uint16_t* u = reinterpret_cast<const uint16_t*>(q);
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+        x[i] = make_uint2(u[16 * i] | (uint32_t)u[16 * i + 1] << 16, u[16 * i + 2] | (uint32_t)u[16 * i + 3] << 16);
+    }
     float top = 0.0f;
-    float x[CH][4];
+    auto value = [&](uint32_t w, int half) {
+      const uint16_t bits = (uint16_t)(w >> (16 * half));
+      return as_float(*reinterpret_cast<const T*>(&bits));
+    };
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
+      if (!in) x[i] = make_uint2(0, 0);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[i][e] = in ? as_float(q[16 * i + 4 * c + e]) : 0.0f;
-        if (fabsf(x[i][e]) < 3.39e38f) top = fmaxf(top, fabsf(x[i][e]));
+        const float z = fabsf(value(e < 2 ? x[i].x : x[i].y, e & 1));
+        if (z < 3.39e38f) top = fmaxf(top, z);
       }
     }
     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
@@ -105,42 +202,19 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
     const float down = __uint_as_float((uint32_t)(254 - e2) << 23), up = __uint_as_float((uint32_t)e2 << 23);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      qf[n][i][0] = pack_half2(x[i][0] * down, x[i][1] * down);
-      qf[n][i][1] = pack_half2(x[i][2] * down, x[i][3] * down);
+      qf[n][i][0] = pack_half2(value(x[i].x, 0) * down, value(x[i].x, 1) * down);
+      qf[n][i][1] = pack_half2(value(x[i].y, 0) * down, value(x[i].y, 1) * down);
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      factor[n][e] = __shfl_sync(0xFFFFFFFFu, up, (2 * c + e) * 4) * a.scale;
+      factor[n][e] = __shfl_sync(0xFFFFFFFFu, up, (2 * c + e) * 4) * a.scale * (CAP ? 1.0f : kLog2e);
       const int rr = 8 * n + 2 * c + e, tt = (row0 + rr) / a.G;
       limit[n][e] = rr < rows ? limit_of(row0 + rr) : 0;
       pos[n][e] = (float)(len - nq + tt);
       slope[n][e] = a.slopes && rr < rows ? a.slopes[h * a.G + row0 + rr - tt * a.G] * kLog2e : 0.0f;
     }
   }
-  const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
-
-  const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * KB;
-  const int32_t* table = a.table + b * a.ld_table;
-  auto page_of = [&](int key) {  // -1: no such page
-    if (key >= key1) return -1;
-    const int page = __ldg(table + key / a.P);
-    return page >= 0 && page < a.pages ? page : -1;
-  };
-  const int64_t head_bytes = (int64_t)a.P * D;
-  auto load = [&](int key, int slot, int p0, int p1) {
-    // keys key .. key + 31, of pages p0 (first sixteen) and p1
-    const uint32_t dst = ring + slot * 2 * KB;
-#pragma unroll
-    for (int i = 0; i < kTile / RPI; ++i) {
-      const int row = i * RPI + lane / LPR, chunk = lane % LPR, kk = key + row;
-      const int page = row < 16 ? p0 : p1;
-      const bool in = kk < key1 && page >= 0;
-      const int64_t off = in ? ((int64_t)page * a.H + h) * head_bytes + (int64_t)(kk % a.P) * D + chunk * 16 : 0;
-      const int sw = D == 64 ? chunk ^ (row >> 1 & 3) : chunk ^ (row & 7);
-      cp_async_16(dst + row * D + sw * 16, a.k + off, in ? 16 : 0);
-      cp_async_16(dst + KB + row * D + sw * 16, a.v + off, in ? 16 : 0);
-    }
-  };
+  const float inv_cap = CAP ? 1.0f / a.cap : 0.0f;
 
   float acc[NT][CH][4] = {};  // output, transposed: elements 16 i + 2 g (c0, c1) and + 1 (c2, c3) of rows 2 c, 2 c + 1
   float run[NT][2], sum[NT][2];
@@ -151,203 +225,147 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
       run[n][e] = -INFINITY;
       sum[n][e] = 0.0f;
     }
-  float vref = 0.0f;
-  constexpr int STEP = kWarps * kTile;
-  int pages[kStages][2];
-  float kss[kStages][2], vss[kStages][2];
-  auto fetch = [&](int key, int s) {
+  int stage = 0, ahead = kStages - 1;
+#pragma unroll 1
+  for (int tile = 0; first + tile * STEP < key1; ++tile) {
+    const int key = first + tile * STEP;
+    fetch(tile + kStages - 1, ahead);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    __syncwarp();
+    const uint32_t kt = ring + stage * 2 * KB, vt = kt + KB;
+    const float4 un[2] = {unit[warp][stage][0], unit[warp][stage][1]};
+    if (++stage == kStages) stage = 0;
+    if (++ahead == kStages) ahead = 0;
+    // scores of two 16-key units
+    float sc[2][NT][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int page = page_of(key + 16 * u);
-      pages[s][u] = page;
-      kss[s][u] = page >= 0 ? __ldg(a.ks + (int64_t)page * a.H + h) : 0.0f;
-      vss[s][u] = page >= 0 ? __ldg(a.vs + (int64_t)page * a.H + h) : 0.0f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[u][n][0] = sc[u][n][1] = sc[u][n][2] = sc[u][n][3] = 0.0f;
+      const int row = 16 * u + (lane & 15);
+#pragma unroll
+      for (int i = 0; i < CH; i += 2) {
+        uint32_t r[4];
+        const int chunk = i + (lane >> 4), sw = D == 64 ? chunk ^ (row >> 1 & 3) : chunk ^ (row & 7);
+        ldsm_x4(kt + row * D + sw * 16, r);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t f[4] = {e4m3x2_f16x2(r[2 * x]), e4m3x2_f16x2(r[2 * x + 1]), e4m3x2_f16x2(r[2 * x] >> 16),
+                                 e4m3x2_f16x2(r[2 * x + 1] >> 16)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(sc[u][n], f, qf[n][i + x][0], qf[n][i + x][1]);
+        }
+      }
     }
-    if (key < key1) load(key, s, pages[s][0], pages[s][1]);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  const int first = key0 + warp * kTile;
+    // to base-2 exponents with the value scale; masked where a row does not reach
+    const bool edge = key + kTile > least || un[0].w < 0.0f || un[1].w < 0.0f;
+    float top[NT][2];
+    bool moves = false;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) fetch(first + s * STEP, s);
-  for (int base = first; base < key1; base += kStages * STEP) {
-#pragma unroll
-    for (int s = 0; s < kStages; ++s) {
-      const int key = base + s * STEP;
-      if (key >= key1) break;
-      fetch(key + (kStages - 1) * STEP, (s + kStages - 1) % kStages);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-      __syncwarp();
-      const uint32_t kt = ring + s * 2 * KB, vt = kt + KB;
-      // scores of two 16-key units
-      float sc[2][NT][4];
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sc[u][n][0] = sc[u][n][1] = sc[u][n][2] = sc[u][n][3] = 0.0f;
-        const int row = 16 * u + (lane & 15);
-#pragma unroll
-        for (int i = 0; i < CH; i += 2) {
-          uint32_t r[4];
-          const int chunk = i + (lane >> 4), sw = D == 64 ? chunk ^ (row >> 1 & 3) : chunk ^ (row & 7);
-          ldsm_x4(kt + row * D + sw * 16, r);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint32_t f[4] = {e4m3x2_f16x2(r[2 * x]), e4m3x2_f16x2(r[2 * x + 1]), e4m3x2_f16x2(r[2 * x] >> 16),
-                                   e4m3x2_f16x2(r[2 * x + 1] >> 16)};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(sc[u][n], f, qf[n][i + x][0], qf[n][i + x][1]);
-          }
+        for (int e = 0; e < 4; ++e) {
+          float x = sc[u][n][e] * (factor[n][e & 1] * un[u].x);
+          if (CAP) x = soft_cap(x, a.cap, inv_cap) * kLog2e;
+          sc[u][n][e] = x + un[u].y;
         }
       }
-      // to base-2 exponents; masked where a row does not reach
-      const bool edge = key + kTile > least || pages[s][0] < 0 || pages[s][1] < 0;
+      if (a.slopes) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = key + 16 * u + g + (e >> 1) * 8;
-            float x = sc[u][n][e] * (factor[n][e & 1] * kss[s][u]);
-            if (a.cap > 0.0f) x = soft_cap(x, a.cap, inv_cap);
-            x *= kLog2e;
-            if (a.slopes) x -= slope[n][e & 1] * fabsf(pos[n][e & 1] - (float)j);
-            if (edge && (j >= limit[n][e & 1] || pages[s][u] < 0)) x = -INFINITY;
-            sc[u][n][e] = x;
-          }
-        }
+          for (int e = 0; e < 4; ++e)
+            sc[u][n][e] = fmaf(-slope[n][e & 1], fabsf(pos[n][e & 1] - (float)(key + 16 * u + g + (e >> 1) * 8)), sc[u][n][e]);
       }
-      // the running maximum moves only when a score passes it by more than kLazy
-      float top[NT][2];
-      bool moves = false;
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key + 16 * u + g + (e >> 1) * 8 >= limit[n][e & 1] || un[u].w < 0.0f) sc[u][n][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[n][e] = fmaxf(fmaxf(sc[0][n][e], sc[0][n][e + 2]), fmaxf(sc[1][n][e], sc[1][n][e + 2]));
+        moves |= top[n][e] > run[n][e] + kLazy;
+      }
+    }
+    // the running maximum moves only when a score passes it by more than kLazy
+    if (__any_sync(0xFFFFFFFFu, moves)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          top[n][e] = fmaxf(fmaxf(sc[0][n][e], sc[0][n][e + 2]), fmaxf(sc[1][n][e], sc[1][n][e + 2]));
-          moves |= top[n][e] > run[n][e] + kLazy;
+          float t = top[n][e];
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 4));
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 8));
+          t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
+          t = fmaxf(t, run[n][e]);
+          f[e] = run[n][e] == -INFINITY ? 0.0f : ex2_approx_ftz(run[n][e] - t);
+          run[n][e] = t;
+          sum[n][e] *= f[e];
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          acc[n][i][0] *= f[0];
+          acc[n][i][1] *= f[1];
+          acc[n][i][2] *= f[0];
+          acc[n][i][3] *= f[1];
         }
       }
-      if (__any_sync(0xFFFFFFFFu, moves)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float f[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float t = top[n][e];
-            t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 4));
-            t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 8));
-            t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
-            t = fmaxf(t, run[n][e]);
-            f[e] = run[n][e] == -INFINITY ? 0.0f : ex2_approx_ftz(run[n][e] - t);
-            run[n][e] = t;
-            sum[n][e] *= f[e];
-          }
-#pragma unroll
-          for (int i = 0; i < CH; ++i) {
-            acc[n][i][0] *= f[0];
-            acc[n][i][1] *= f[1];
-            acc[n][i][2] *= f[0];
-            acc[n][i][3] *= f[1];
-          }
-        }
-      }
-      // weights
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float m = run[n][e & 1];
-            sc[u][n][e] = ex2_approx_ftz(sc[u][n][e] - (m == -INFINITY ? 0.0f : m));
-            sum[n][e & 1] += sc[u][n][e];
-          }
-        }
-      }
-      uint32_t seen[2][NT][2];
-      // A NaN among the values of a tile that some row sees only in part: it belongs to the rows that see it alone
-      bool nan_here = false;
-      if (edge) {
-        for (int i = lane; i < KB / 16; i += 32) {
-          uint4 x;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(vt + i * 16));
-          const uint32_t z[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) nan_here |= __vcmpeq4(z[e] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
-        }
-        nan_here = __any_sync(0xFFFFFFFFu, nan_here);
-        if (nan_here) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              float see[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) see[e] = key + 16 * u + g + (e >> 1) * 8 < limit[n][e & 1] ? 1.0f : 0.0f;
-              seen[u][n][0] = transpose8x8(pack_half2(see[0], see[1]));
-              seen[u][n][1] = transpose8x8(pack_half2(see[2], see[3]));
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        // the output is kept in units of vref: another page's scale goes into the weights, within what f16 takes
-        float ratio = 0.0f;
-        if (pages[s][u] >= 0) {
-          if (vref == 0.0f) vref = vss[s][u];
-          ratio = vref == 0.0f ? 0.0f : __fdividef(vss[s][u], vref);
-          if (ratio != 0.0f && (ratio > 64.0f || ratio < 0.015625f)) {
-            const float f = fminf(vref / vss[s][u], 1e38f);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int i = 0; i < CH; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[n][i][e] *= f;
-            vref = vss[s][u];
-            ratio = 1.0f;
-          }
-        }
-        // 16 keys x 8 rows transposed into the MMA's B fragments
-        uint32_t w[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          w[n][0] = transpose8x8(pack_half2(sc[u][n][0] * ratio, sc[u][n][1] * ratio));
-          w[n][1] = transpose8x8(pack_half2(sc[u][n][2] * ratio, sc[u][n][3] * ratio));
-        }
-        const int row = 16 * u + (lane & 15);
-#pragma unroll
-        for (int i = 0; i < CH; i += 2) {
-          uint32_t r[4];
-          const int chunk = i + (lane >> 4), sw = D == 64 ? chunk ^ (row >> 1 & 3) : chunk ^ (row & 7);
-          ldsm_x4_trans(vt + row * D + sw * 16, r);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            // a register has two elements of two neighbouring keys: pair the keys
-            const uint32_t lo = __byte_perm(r[2 * x], 0, 0x3120), hi = __byte_perm(r[2 * x + 1], 0, 0x3120);
-            uint32_t f[4] = {e4m3x2_f16x2(lo), e4m3x2_f16x2(lo >> 16), e4m3x2_f16x2(hi), e4m3x2_f16x2(hi >> 16)};
-            if (nan_here) {
-              const uint32_t at[4] = {nan_halves(f[0]), nan_halves(f[1]), nan_halves(f[2]), nan_halves(f[3])};
-#pragma unroll
-              for (int z = 0; z < 4; ++z) f[z] = without_nan(f[z]);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                float hits[4] = {};
-                mma_f16(hits, at, seen[u][n][0], seen[u][n][1]);
-#pragma unroll
-                for (int z = 0; z < 4; ++z)
-                  if (hits[z] > 0.0f) acc[n][i + x][z] = __uint_as_float(0x7FC00000u);
-              }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(acc[n][i + x], f, w[n][0], w[n][1]);
-          }
-        }
-      }
-      __syncwarp();
     }
+    // A NaN among the values of a tile that some row sees only in part belongs to the rows that see it alone.
+    if (edge) {
+      bool nan_here = false;
+#pragma unroll 1
+      for (int i = lane; i < KB / 16; i += 32) {
+        uint4 x;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(vt + i * 16));
+        nan_here |= (__vcmpeq4(x.x & 0x7F7F7F7Fu, 0x7F7F7F7Fu) | __vcmpeq4(x.y & 0x7F7F7F7Fu, 0x7F7F7F7Fu) |
+                     __vcmpeq4(x.z & 0x7F7F7F7Fu, 0x7F7F7F7Fu) | __vcmpeq4(x.w & 0x7F7F7F7Fu, 0x7F7F7F7Fu)) != 0;
+      }
+      if (__any_sync(0xFFFFFFFFu, nan_here)) take_nans(vt, KB, D, key, lane, first_nan);
+    }
+    // weights, 16 keys x 8 rows transposed into the MMA's B fragments, and their product with the codes
+    uint32_t w[2][NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float m[2] = {run[n][0] == -INFINITY ? 0.0f : run[n][0], run[n][1] == -INFINITY ? 0.0f : run[n][1]};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = ex2_approx_ftz(sc[u][n][e] - m[e & 1]);
+          sum[n][e & 1] = fmaf(p[e], un[u].z, sum[n][e & 1]);
+        }
+        const bool nil = un[u].w == 0.0f;
+        w[u][n][0] = transpose8x8(nil ? 0u : pack_half2(p[0], p[1]));
+        w[u][n][1] = transpose8x8(nil ? 0u : pack_half2(p[2], p[3]));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = 16 * u + (lane & 15);
+#pragma unroll
+      for (int i = 0; i < CH; i += 2) {
+        uint32_t r[4];
+        const int chunk = i + (lane >> 4), sw = D == 64 ? chunk ^ (row >> 1 & 3) : chunk ^ (row & 7);
+        ldsm_x4_trans(vt + row * D + sw * 16, r);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          // a register has two elements of two neighbouring keys: pair the keys
+          const uint32_t lo = __byte_perm(r[2 * x], 0, 0x3120), hi = __byte_perm(r[2 * x + 1], 0, 0x3120);
+          const uint32_t f[4] = {e4m3x2_f16x2(lo), e4m3x2_f16x2(lo >> 16), e4m3x2_f16x2(hi), e4m3x2_f16x2(hi >> 16)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(acc[n][i + x], f, w[u][n][0], w[u][n][1]);
+        }
+      }
+    }
+    __syncwarp();
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   grid_launch_dependents();
@@ -371,17 +389,17 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
       }
 #pragma unroll
       for (int i = 0; i < CH; ++i)
-        *reinterpret_cast<float2*>(part + (warp * ROWS + r) * LD + 16 * i + 2 * g) =
-            make_float2(acc[n][i][e] * vref, acc[n][i][e + 2] * vref);
+        *reinterpret_cast<float2*>(part + (warp * ROWS + r) * LD + 16 * i + 2 * g) = make_float2(acc[n][i][e], acc[n][i][e + 2]);
     }
   }
   __syncthreads();
   const int ticket = b * a.H * a.row_tiles + y;
-  T* out = reinterpret_cast<T*>(a.out);
+  T* out = reinterpret_cast<T*>(a.out) + b * a.o_b;
   auto out_row = [&](int r) {
     const int t = (row0 + r) / a.G, hq = h * a.G + (row0 + r) - t * a.G;
-    return out + b * a.o_b + t * a.o_t + hq * a.o_h;
+    return out + t * a.o_t + hq * a.o_h;
   };
+#pragma unroll 1
   for (int i = threadIdx.x; i < rows * D; i += 32 * kWarps) {
     const int r = i / D, d = i - r * D;
     float m = -INFINITY;
@@ -390,10 +408,11 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
     float l = 0.0f, o = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = m_of[w][r] == -INFINITY ? 0.0f : ex2_approx_ftz(m_of[w][r] - m);
-      l += m_of[w][r] == -INFINITY ? l_of[w][r] : f * l_of[w][r];
-      o += m_of[w][r] == -INFINITY ? part[(w * ROWS + r) * LD + d] : f * part[(w * ROWS + r) * LD + d];
+      const float f = m_of[w][r] == -INFINITY ? 1.0f : ex2_approx_ftz(m_of[w][r] - m);
+      l = fmaf(f, l_of[w][r], l);
+      o = fmaf(f, part[(w * ROWS + r) * LD + d], o);
     }
+    if (first_nan[d] < limits[r]) o = __uint_as_float(0x7FC00000u);
     if (chunks == 1) {
       put(out_row(r) + d, l == 0.0f ? 0.0f : o / l);
     } else {
@@ -413,23 +432,26 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
   if (threadIdx.x == 0) a.tickets[ticket] = 0;
   const float2* ml = reinterpret_cast<const float2*>(a.partial + a.partial_ml) + (int64_t)ticket * a.splits * ROWS;
   const float* po = a.partial + (int64_t)ticket * a.splits * ROWS * D;
+#pragma unroll 1
   for (int i = threadIdx.x; i < rows * D; i += 32 * kWarps) {
     const int r = i / D, d = i - r * D;
     float m = -INFINITY;
+#pragma unroll 4
     for (int s = 0; s < chunks; ++s) m = fmaxf(m, __ldcg(ml + s * ROWS + r).x);
     float l = 0.0f, o = 0.0f;
+#pragma unroll 4
     for (int s = 0; s < chunks; ++s) {
       const float2 x = __ldcg(ml + s * ROWS + r);
       const float f = x.x == -INFINITY ? 1.0f : ex2_approx_ftz(x.x - m);
-      l += f * x.y;
-      o += f * __ldcg(po + ((int64_t)s * ROWS + r) * D + d);
+      l = fmaf(f, x.y, l);
+      o = fmaf(f, __ldcg(po + ((int64_t)s * ROWS + r) * D + d), o);
     }
     put(out_row(r) + d, l == 0.0f ? 0.0f : o / l);
   }
 }
 
-template <int D, int NT, typename T>
-int launch_rows(const AttendArgs& a, cudaStream_t s) {
+template <int D, int NT, typename T, bool CAP>
+int launch_rows(const AttendArgs& a, int vec, cudaStream_t s) {
   constexpr int ring = kWarps * kStages * 2 * kTile * D, meet = kWarps * 8 * NT * (D + 8) * 4;
   constexpr int smem = ring > meet ? ring : meet;
   static bool attr_set[64] = {};
@@ -438,14 +460,21 @@ int launch_rows(const AttendArgs& a, cudaStream_t s) {
   if (dev < 0 || dev >= 64) return IFLB200_ERR_DEVICE;
   if (!attr_set[dev]) {
     const cudaError_t e =
-        cudaFuncSetAttribute(cache_attend_rows_kernel<D, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaFuncSetAttribute(cache_attend_rows_kernel<D, NT, T, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
     attr_set[dev] = true;
   }
   const dim3 grid((unsigned)a.splits, (unsigned)(a.H * a.row_tiles), (unsigned)a.B);
-  const cudaError_t e = launch_dep(cache_attend_rows_kernel<D, NT, T>, grid, dim3(32 * kWarps), smem, s, 1,
-                                   dependent_launch_for((int64_t)a.B * a.T), a);
+  const cudaError_t e = launch_dep(cache_attend_rows_kernel<D, NT, T, CAP>, grid, dim3(32 * kWarps), smem, s, 1,
+                                   dependent_launch_for((int64_t)a.B * a.T), a, vec);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+template <int D, int NT, typename T>
+int launch_rows(const AttendArgs& a, cudaStream_t s) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)((a.q_b | a.q_t | a.q_h) * (int64_t)sizeof(T));
+  const int vec = bits % 8 == 0;
+  return a.cap > 0.0f ? launch_rows<D, NT, T, true>(a, vec, s) : launch_rows<D, NT, T, false>(a, vec, s);
 }
 
 // iflb200_cache_attention_set_form; 0: by rule
@@ -472,6 +501,7 @@ int attend(AttendArgs a, int D, void* workspace, int64_t bytes, cudaStream_t s) 
   const int64_t each = units * per * (D + 2) * 4;
   const int64_t room = workspace && bytes > head ? (bytes - head) / each : 0;
   int64_t splits = units * 4 > head ? 1 : (want < room ? want : room);
+  if (many && splits > 64) splits = 64;  // (shares of the chunks are added up in shared memory)
   if (splits < 1) splits = 1;
   int64_t chunk = ((keys + splits - 1) / splits + kLeast - 1) / kLeast * kLeast;
   if (chunk < kLeast) chunk = kLeast;

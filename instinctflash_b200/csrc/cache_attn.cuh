@@ -49,6 +49,11 @@ __device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 
+__device__ __forceinline__ float log2_approx(float a) {
+  float r;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(a));
+  return r;
+}
 // Two e4m3 codes in the low half of `two` as two f16 (exact).
 __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two) {
   uint32_t r;

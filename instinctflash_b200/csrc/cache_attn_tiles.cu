@@ -103,11 +103,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float log2_approx(float a) {
-  float r;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(a));
-  return r;
-}
 __device__ __forceinline__ float row_value(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float row_value(__half x) { return __half2float(x); }
 template <typename T>
@@ -457,48 +452,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     }
     if (chunks > 1) {
       if (in) *reinterpret_cast<float2*>(a.partial + a.partial_ml + at * 2) = make_float2(top_run, l);
-      // the last CTA of the chunks adds them up, in their order
+      // the last CTA of the chunks adds them up (below)
       __threadfence();
       named_bar_sync(1, 128 * NQ);
       if (threadIdx.x == 128) *last_one = atomicAdd(a.tickets + ticket, 1u) == (uint32_t)chunks - 1;
-      named_bar_sync(1, 128 * NQ);
-      if (*last_one) {
-        __threadfence();
-        if (threadIdx.x == 128) a.tickets[ticket] = 0;
-        const int64_t from = (int64_t)ticket * a.splits * L::ROWS;
-        const float2* ml = reinterpret_cast<const float2*>(a.partial + a.partial_ml) + from;
-        const float* po = a.partial + from * D;
-        for (int i = threadIdx.x - 128; i < rows * (D / 4); i += 128 * NQ) {
-          const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4;
-          float mm = -INFINITY;
-          for (int s = 0; s < chunks; ++s) mm = fmaxf(mm, __ldcg(ml + s * L::ROWS + rr).x);
-          float ll = 0.0f;
-          float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int s = 0; s < chunks; ++s) {
-            const float2 x = __ldcg(ml + s * L::ROWS + rr);
-            const float f = x.x == -INFINITY ? 1.0f : ex2_approx_ftz(x.x - mm);
-            const float4 u = __ldcg(reinterpret_cast<const float4*>(po + ((int64_t)s * L::ROWS + rr) * D + d));
-            ll += f * x.y;
-            o.x += f * u.x;
-            o.y += f * u.y;
-            o.z += f * u.z;
-            o.w += f * u.w;
-          }
-          const float w = ll == 0.0f ? 0.0f : 1.0f / ll;
-          const int t2 = (row0 + rr) / a.G, h2 = h * a.G + (row0 + rr) - t2 * a.G;
-          T* dst = reinterpret_cast<T*>(a.out) + b * a.o_b + t2 * a.o_t + h2 * a.o_h + d;
-          const uint32_t w0 = pack_out<T>(o.x * w, o.y * w), w1 = pack_out<T>(o.z * w, o.w * w);
-          if (vec) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
-          } else {
-            const T *p0 = reinterpret_cast<const T*>(&w0), *p1 = reinterpret_cast<const T*>(&w1);
-            dst[0] = p0[0];
-            dst[1] = p0[1];
-            dst[2] = p1[0];
-            dst[3] = p1[1];
-          }
-        }
-      }
     }
   } else if (warp >= 12) {
     // ------------------------------------------------------------------ codes to f16 tiles
@@ -663,6 +620,55 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+  if (chunks == 1 || !*last_one) return;
+  // All threads, in the order of the chunks: first every row's share of each, then the sums, several loads in flight.
+  __threadfence();
+  const int ticket = b * a.H * a.row_tiles + y;
+  if (threadIdx.x == 0) a.tickets[ticket] = 0;
+  const int64_t from = (int64_t)ticket * a.splits * L::ROWS;
+  const float2* ml = reinterpret_cast<const float2*>(a.partial + a.partial_ml) + from;
+  const float* po = a.partial + from * D;
+  float* share = reinterpret_cast<float*>(smem);  // [chunk][row]: the operands' shared memory is free
+  for (int r = threadIdx.x; r < rows; r += kThreads) {
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < chunks; ++s) m = fmaxf(m, __ldcg(ml + s * L::ROWS + r).x);
+#pragma unroll 4
+    for (int s = 0; s < chunks; ++s) {
+      const float2 x = __ldcg(ml + s * L::ROWS + r);
+      const float f = x.x == -INFINITY ? 1.0f : ex2_approx_ftz(x.x - m);
+      share[s * L::ROWS + r] = f;
+      l = fmaf(f, x.y, l);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int s = 0; s < chunks; ++s) share[s * L::ROWS + r] *= inv;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int s = 0; s < chunks; ++s) {
+      const float f = share[s * L::ROWS + r];
+      const float4 u = __ldcg(reinterpret_cast<const float4*>(po + ((int64_t)s * L::ROWS + r) * D + d));
+      o.x = fmaf(f, u.x, o.x);
+      o.y = fmaf(f, u.y, o.y);
+      o.z = fmaf(f, u.z, o.z);
+      o.w = fmaf(f, u.w, o.w);
+    }
+    const int t = (row0 + r) / a.G, hq = h * a.G + (row0 + r) - t * a.G;
+    T* dst = reinterpret_cast<T*>(a.out) + b * a.o_b + t * a.o_t + hq * a.o_h + d;
+    const uint32_t w0 = pack_out<T>(o.x, o.y), w1 = pack_out<T>(o.z, o.w);
+    if (vec) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
+    } else {
+      const T *p0 = reinterpret_cast<const T*>(&w0), *p1 = reinterpret_cast<const T*>(&w1);
+      dst[0] = p0[0];
+      dst[1] = p0[1];
+      dst[2] = p1[0];
+      dst[3] = p1[1];
+    }
   }
 }
 
