@@ -13,7 +13,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kTile = 32;    // keys a warp takes at a time
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -37,11 +37,30 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+// Four elements of a row; `vec`: rows are 8-byte aligned.
+template <typename T>
+__device__ __forceinline__ void put4(T* p, float a, float b, float c, float d, int vec) {
+  T x[4];
+  put(x, a);
+  put(x + 1, b);
+  put(x + 2, c);
+  put(x + 3, d);
+  if (vec) {
+    uint2 u;
+    u.x = *reinterpret_cast<const uint16_t*>(x) | (uint32_t)*reinterpret_cast<const uint16_t*>(x + 1) << 16;
+    u.y = *reinterpret_cast<const uint16_t*>(x + 2) | (uint32_t)*reinterpret_cast<const uint16_t*>(x + 3) << 16;
+    *reinterpret_cast<uint2*>(p) = u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = x[i];
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // Few rows (query token x head of a group): bound by the cache's bytes.
 //
 // Keys on the MMA's M side, 8 rows on its N side.  Every warp walks key tiles of its own with a softmax state of its
-// own, loads (cp.async, two tiles ahead, 16-byte pieces swizzled for ldmatrix) and all: no barrier until the end.
+// own, loads (cp.async, one tile ahead, 16-byte pieces swizzled for ldmatrix) and all: no barrier until the end.
 // Codes become f16 in registers, which is exact; q is f16 too, its row brought near 1 by a power of two (a bf16 row keeps
 // all its bits down to 2^-14 of its largest element); weights are f16 relative to the row's running maximum.  All sums
 // and the softmax state are fp32.
@@ -399,25 +418,36 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
     const int t = (row0 + r) / a.G, hq = h * a.G + (row0 + r) - t * a.G;
     return out + t * a.o_t + hq * a.o_h;
   };
+  // four elements of a row a thread
 #pragma unroll 1
-  for (int i = threadIdx.x; i < rows * D; i += 32 * kWarps) {
-    const int r = i / D, d = i - r * D;
-    float m = -INFINITY;
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kWarps) {
+    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) m = fmaxf(m, m_of[w][r]);
-    float l = 0.0f, o = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float f = m_of[w][r] == -INFINITY ? 1.0f : ex2_approx_ftz(m_of[w][r] - m);
+      const float4 x = *reinterpret_cast<const float4*>(part + (w * ROWS + r) * LD + d);
       l = fmaf(f, l_of[w][r], l);
-      o = fmaf(f, part[(w * ROWS + r) * LD + d], o);
+      o.x = fmaf(f, x.x, o.x);
+      o.y = fmaf(f, x.y, o.y);
+      o.z = fmaf(f, x.z, o.z);
+      o.w = fmaf(f, x.w, o.w);
     }
-    if (first_nan[d] < limits[r]) o = __uint_as_float(0x7FC00000u);
+    const int lim = limits[r];
+    const float nan = __uint_as_float(0x7FC00000u);
+    if (first_nan[d] < lim) o.x = nan;
+    if (first_nan[d + 1] < lim) o.y = nan;
+    if (first_nan[d + 2] < lim) o.z = nan;
+    if (first_nan[d + 3] < lim) o.w = nan;
     if (chunks == 1) {
-      put(out_row(r) + d, l == 0.0f ? 0.0f : o / l);
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      put4(out_row(r) + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv, vec);
     } else {
       const int64_t at = ((int64_t)ticket * a.splits + split) * ROWS + r;
-      a.partial[at * D + d] = o;
+      *reinterpret_cast<float4*>(a.partial + at * D + d) = o;
       if (d == 0) *reinterpret_cast<float2*>(a.partial + a.partial_ml + at * 2) = make_float2(m, l);
     }
   }
@@ -430,23 +460,52 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
   if (!last_one) return;
   __threadfence();
   if (threadIdx.x == 0) a.tickets[ticket] = 0;
+  // every row's share of each chunk first, then the sums, four elements a thread and several chunks in flight
   const float2* ml = reinterpret_cast<const float2*>(a.partial + a.partial_ml) + (int64_t)ticket * a.splits * ROWS;
   const float* po = a.partial + (int64_t)ticket * a.splits * ROWS * D;
-#pragma unroll 1
-  for (int i = threadIdx.x; i < rows * D; i += 32 * kWarps) {
-    const int r = i / D, d = i - r * D;
-    float m = -INFINITY;
+  float* share = part;  // [chunk][row]
+  if (threadIdx.x < 8 * ROWS) {  // eight lanes a row
+    const int r = threadIdx.x >> 3, at = threadIdx.x & 7;
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll 4
-    for (int s = 0; s < chunks; ++s) m = fmaxf(m, __ldcg(ml + s * ROWS + r).x);
-    float l = 0.0f, o = 0.0f;
+    for (int s = at; s < chunks; s += 8) m = fmaxf(m, __ldcg(ml + s * ROWS + r).x);
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
 #pragma unroll 4
-    for (int s = 0; s < chunks; ++s) {
+    for (int s = at; s < chunks; s += 8) {
       const float2 x = __ldcg(ml + s * ROWS + r);
       const float f = x.x == -INFINITY ? 1.0f : ex2_approx_ftz(x.x - m);
+      share[s * ROWS + r] = f;
       l = fmaf(f, x.y, l);
-      o = fmaf(f, __ldcg(po + ((int64_t)s * ROWS + r) * D + d), o);
     }
-    put(out_row(r) + d, l == 0.0f ? 0.0f : o / l);
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int s = at; s < chunks; s += 8) share[s * ROWS + r] *= inv;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kWarps) {
+    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int s0 = 0; s0 < chunks; s0 += 8) {
+      float4 u[8];
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        if (s0 + z < chunks) u[z] = __ldcg(reinterpret_cast<const float4*>(po + ((int64_t)(s0 + z) * ROWS + r) * D + d));
+#pragma unroll
+      for (int z = 0; z < 8; ++z) {
+        if (s0 + z < chunks) {
+          const float f = share[(s0 + z) * ROWS + r];
+          o.x = fmaf(f, u[z].x, o.x);
+          o.y = fmaf(f, u[z].y, o.y);
+          o.z = fmaf(f, u[z].z, o.z);
+          o.w = fmaf(f, u[z].w, o.w);
+        }
+      }
+    }
+    put4(out_row(r) + d, o.x, o.y, o.z, o.w, vec);
   }
 }
 
@@ -472,7 +531,8 @@ int launch_rows(const AttendArgs& a, int vec, cudaStream_t s) {
 
 template <int D, int NT, typename T>
 int launch_rows(const AttendArgs& a, cudaStream_t s) {
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)((a.q_b | a.q_t | a.q_h) * (int64_t)sizeof(T));
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) |
+                         (uintptr_t)((a.q_b | a.q_t | a.q_h | a.o_b | a.o_t | a.o_h) * (int64_t)sizeof(T));
   const int vec = bits % 8 == 0;
   return a.cap > 0.0f ? launch_rows<D, NT, T, true>(a, vec, s) : launch_rows<D, NT, T, false>(a, vec, s);
 }
@@ -491,17 +551,18 @@ int attend(AttendArgs a, int D, void* workspace, int64_t bytes, cudaStream_t s) 
   a.row_tiles = (int)tiles;
   const int sms = device_sm_count();
   if (sms == 0) return IFLB200_ERR_DEVICE;
-  // Chunks of keys: enough for two waves of CTAs, none shorter than a step of all warps, as many as the workspace takes.
+  // Chunks of keys: enough for some waves of CTAs, none shorter than a step of all warps, as many as the workspace takes.
   const int64_t keys = (int64_t)a.max_pages * a.P, units = (int64_t)a.B * a.H * tiles;
   constexpr int64_t kLeast = kWarps * kTile;
-  const int64_t want = ((many ? 1ll : 4ll) * sms + units - 1) / units;
+  const int64_t want = ((many ? 1ll : 8ll) * sms + units - 1) / units;
   // The tickets have a place of their own whatever the geometry: they are zero between calls, partial results are not.
   // (Sequences are only shared where there are fewer units than CTAs wanted.)
   constexpr int64_t head = 4096;
   const int64_t each = units * per * (D + 2) * 4;
   const int64_t room = workspace && bytes > head ? (bytes - head) / each : 0;
   int64_t splits = units * 4 > head ? 1 : (want < room ? want : room);
-  if (many && splits > 64) splits = 64;  // (shares of the chunks are added up in shared memory)
+  const int64_t most = many ? 64 : 512;  // (shares of the chunks are worked out in shared memory)
+  if (splits > most) splits = most;
   if (splits < 1) splits = 1;
   int64_t chunk = ((keys + splits - 1) / splits + kLeast - 1) / kLeast * kLeast;
   if (chunk < kLeast) chunk = kLeast;
