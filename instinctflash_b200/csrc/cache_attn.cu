@@ -561,8 +561,7 @@ int attend(AttendArgs a, int D, void* workspace, int64_t bytes, cudaStream_t s) 
   const int64_t each = units * per * (D + 2) * 4;
   const int64_t room = workspace && bytes > head ? (bytes - head) / each : 0;
   int64_t splits = units * 4 > head ? 1 : (want < room ? want : room);
-  const int64_t most = many ? 64 : 512;  // (shares of the chunks are worked out in shared memory)
-  if (splits > most) splits = most;
+  if (splits > 512) splits = 512;  // (shares of the chunks are worked out in shared memory)
   if (splits < 1) splits = 1;
   int64_t chunk = ((keys + splits - 1) / splits + kLeast - 1) / kLeast * kLeast;
   if (chunk < kLeast) chunk = kLeast;

@@ -44,7 +44,8 @@ struct Tiles {
   static constexpr int kNan = kMeta + 4 * GR * 16;
   static constexpr int kOff = kNan + D * 4 + 16;          // each converter warp's units of two steps: offset of the codes
   static constexpr int kHole = kOff + kConvert * 2 * GR * 8;  // of four steps: whether a unit has no page
-  static constexpr int kBar = kHole + 16;
+  static constexpr int kFactor = kHole + 16;              // of each row of q
+  static constexpr int kBar = kFactor + ROWS * 4;
   static constexpr int kSmem = kBar + 24 * 8 + 16 + 1024;
 };
 
@@ -117,20 +118,6 @@ __device__ __forceinline__ uint32_t pack_out<__half>(float a, float b) {
   return pack_half2(a, b);
 }
 
-// D elements of a row of q: 16 bytes at a time where they are aligned.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_row8(const T* q, float (&x)[8]) {
-  if (VEC) {
-    const uint4 u = *reinterpret_cast<const uint4*>(q);
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = row_value(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = row_value(q[i]);
-  }
-}
-
 // Sixteen codes of key `key` without their NaNs, whose columns learn of the first key that has one.  (Out of line: it is
 // hardly ever run.)
 __device__ __noinline__ uint4 without_nans(uint4 codes, int* first_nan, int key) {
@@ -162,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   const uint32_t q_at = base, k_at = base + NQ * L::kQ, v_at = k_at + 2 * L::kTile, meta = base + L::kMeta, bar0 = base + L::kBar;
   int* nan_at = reinterpret_cast<int*>(smem + L::kNan);  // for each element of D the first key whose value is a NaN there
   volatile int* nan_any = nan_at + D;
-  volatile int* last_one = nan_at + D + 1;
+  float* row_factor = reinterpret_cast<float*>(smem + L::kFactor);
   enum { KFULL = 0, KEMPTY = 2, VFULL = 4, VEMPTY = 6, SFULL = 8, PFULL = 10, PV = 12, QFULL = 14 };
   auto bar = [&](int kind, int i) { return bar0 + 8u * (kind + i); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kBar + 24 * 8);
@@ -195,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
       mbar_init(bar(PFULL, i), 4);
       mbar_init(bar(PV, i), 1);
     }
-    mbar_init(bar(QFULL, 0), 4 * NQ);
+    mbar_init(bar(QFULL, 0), 8);
     tmem_slot[1] = 0;
     *nan_any = 0;
     fence_barrier_init();
@@ -212,6 +199,54 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  if (warp >= 4 && warp < 12) {
+    // The rows of q as f16, each row's largest element near 1: eight warps, LR lanes a row, eight loads in flight.
+    constexpr int LR = D / 8, RI = 32 / LR, RW = L::ROWS / 8;
+    const int piece = lane % LR, from = (warp - 4) * RW;
+#pragma unroll 1
+    for (int i0 = 0; i0 < RW; i0 += 8 * RI) {
+      uint4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int rr = from + i0 + i * RI + lane / LR, row = row0 + (rr < rows ? rr : 0);
+        const int t = row / a.G;
+        const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_b + t * a.q_t + (h * a.G + row - t * a.G) * a.q_h + 8 * piece;
+        if (vec) {
+          x[i] = *reinterpret_cast<const uint4*>(q);
+        } else {
+          const uint16_t* u = reinterpret_cast<const uint16_t*>(q);
+          x[i] = make_uint4(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16, u[6] | (uint32_t)u[7] << 16);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float v[8], top = 0.0f;
+        const T* e8 = reinterpret_cast<const T*>(&x[i]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = row_value(e8[e]);
+          if (fabsf(v[e]) < 3.39e38f) top = fmaxf(top, fabsf(v[e]));
+        }
+        if (LR == 32) {
+          top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top)));
+        } else {
+#pragma unroll
+          for (int z = 1; z < LR; z <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, z));
+        }
+        const int e2 = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
+        const float down = __uint_as_float((uint32_t)(254 - e2) << 23);
+        const int rr = from + i0 + i * RI + lane / LR, r128 = rr & 127;
+        if (piece == 0) row_factor[rr] = __uint_as_float((uint32_t)e2 << 23) * a.scale;
+        sts128(q_at + (rr >> 7) * L::kQ + (piece >> 3) * 128 * 128 + r128 * 128 + (((piece & 7) ^ (r128 & 7)) << 4),
+               pack_half2(v[0] * down, v[1] * down), pack_half2(v[2] * down, v[3] * down), pack_half2(v[4] * down, v[5] * down),
+               pack_half2(v[6] * down, v[7] * down));
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(QFULL, 0));
+    named_bar_sync(1, 256);
+  }
   if (warp >= 4 && warp < 4 + 4 * NQ) {
     // ------------------------------------------------------------------ softmax and output
     const int slot = (warp >> 2) - 1;
@@ -223,36 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     const float pos = (float)(len - nq + tok);
     const float slope = SLOPES ? a.slopes[hq] * kLog2e : 0.0f;
     const float inv_cap = CAP ? 1.0f / a.cap : 0.0f;
-    float factor;
-    {
-      // the row of q as f16, its largest element near 1
-      const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_b + tok * a.q_t + hq * a.q_h;
-      float top = 0.0f;
-#pragma unroll 1
-      for (int i = 0; i < D / 8; ++i) {
-        float x[8];
-        if (vec) load_row8<T, true>(q + 8 * i, x);
-        else load_row8<T, false>(q + 8 * i, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (fabsf(x[e]) < 3.39e38f) top = fmaxf(top, fabsf(x[e]));
-      }
-      const int e2 = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
-      const float down = __uint_as_float((uint32_t)(254 - e2) << 23);
-      factor = __uint_as_float((uint32_t)e2 << 23) * a.scale;
-      const uint32_t at = q_at + slot * L::kQ + (r & 127) * 128;
-#pragma unroll 1
-      for (int i = 0; i < D / 8; ++i) {
-        float x[8];
-        if (vec) load_row8<T, true>(q + 8 * i, x);
-        else load_row8<T, false>(q + 8 * i, x);
-        sts128(at + (i >> 3) * 128 * 128 + (((i & 7) ^ (r & 7)) << 4), pack_half2(x[0] * down, x[1] * down),
-               pack_half2(x[2] * down, x[3] * down), pack_half2(x[4] * down, x[5] * down), pack_half2(x[6] * down, x[7] * down));
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(QFULL, 0));
-    }
+    const float factor = row_factor[r];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_at = tmem + lanes + kO + slot * D;
     float top_run = -INFINITY, l = 0.0f;
@@ -402,61 +408,68 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     }
     if (ok && steps > 0) ok = wait_warp(bar(PV, slot), (steps - 1) & 1u, abort_flag, (1u << 24) | (3u << 16));
     tc_fence_after();
-    const int ticket = b * a.H * a.row_tiles + y;
-    const bool any_nan = *nan_any != 0;
-    const float inv = drop * (chunks > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l));  // (the last move of the maximum is still to be made)
-    T* out = reinterpret_cast<T*>(a.out) + b * a.o_b + tok * a.o_t + hq * a.o_h;
-    const int64_t at = ((int64_t)ticket * a.splits + split) * L::ROWS + r;
-    float* part = a.partial + at * D;
+    // The output through shared memory (this row tile of q is done with), 2 D bytes of each row at a time: whole rows go to
+    // memory, where a row a thread would write half sectors.
+    const bool any_nan = *nan_any != 0, partial = chunks > 1;
+    const float inv = drop * (partial ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l));  // (the last move of the maximum is still to be made)
+    const uint32_t stage = q_at + slot * L::kQ + (warp & 3) * 32 * 2 * D;
+    const int64_t at = ((int64_t)(b * a.H * a.row_tiles + y) * a.splits + split) * L::ROWS;
+    constexpr int PR = D / 8;  // 16-byte pieces of a row
 #pragma unroll 1
-    for (int i = 0; i < D / 16; ++i) {
-      uint32_t o[16];
-      if (steps > 0) {
-        tmem_ld_16c(o_at + 16 * i, o);
-        tmem_ld_wait();
-      } else {
+    for (int pass = 0; pass < (partial ? 2 : 1); ++pass) {
+      __syncwarp();
+#pragma unroll 1
+      for (int i = 0; i < (partial ? D / 32 : D / 16); ++i) {
+        const int col = pass * (D / 2) + 16 * i;
+        uint32_t o[16];
+        if (steps > 0) {
+          tmem_ld_16c(o_at + col, o);
+          tmem_ld_wait();
+        } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = 0;
-      }
-      if (in && ok) {
+          for (int e = 0; e < 16; ++e) o[e] = 0;
+        }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float x = __uint_as_float(o[e]) * inv;
-          if (any_nan && nan_at[16 * i + e] < limit) x = __uint_as_float(0x7FC00000u);
+          if (any_nan && nan_at[col + e] < limit) x = __uint_as_float(0x7FC00000u);
           o[e] = __float_as_uint(x);
         }
-        if (chunks > 1) {
+        const uint32_t row_at = stage + lane * 2 * D;
+        if (partial) {
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<uint4*>(part + 16 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        } else if (vec) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 8) {
-            uint4 u;
-            uint32_t* w = reinterpret_cast<uint32_t*>(&u);
-#pragma unroll
-            for (int z = 0; z < 4; ++z) w[z] = pack_out<T>(__uint_as_float(o[e + 2 * z]), __uint_as_float(o[e + 2 * z + 1]));
-            *reinterpret_cast<uint4*>(out + 16 * i + e) = u;
-          }
+          for (int z = 0; z < 4; ++z) sts128(row_at + (((4 * i + z) ^ (lane & 7)) << 4), o[4 * z], o[4 * z + 1], o[4 * z + 2], o[4 * z + 3]);
         } else {
+          uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const uint32_t w = pack_out<T>(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
-            const T* two = reinterpret_cast<const T*>(&w);
-            out[16 * i + e] = two[0];
-            out[16 * i + e + 1] = two[1];
+          for (int z = 0; z < 8; ++z) w[z] = pack_out<T>(__uint_as_float(o[2 * z]), __uint_as_float(o[2 * z + 1]));
+#pragma unroll
+          for (int z = 0; z < 2; ++z) sts128(row_at + (((2 * i + z) ^ (lane & 7)) << 4), w[4 * z], w[4 * z + 1], w[4 * z + 2], w[4 * z + 3]);
+        }
+      }
+      __syncwarp();
+#pragma unroll 4
+      for (int i = lane; i < 32 * PR; i += 32) {
+        const int rw = i / PR, piece = i % PR, rr = slot * 128 + (warp & 3) * 32 + rw;
+        const float4 f = lds_f4(stage + rw * 2 * D + ((piece ^ (rw & 7)) << 4));
+        if (rr < rows && ok) {
+          if (partial) {
+            *reinterpret_cast<float4*>(a.partial + (at + rr) * D + pass * (D / 2) + piece * 4) = f;
+          } else {
+            const int t = (row0 + rr) / a.G;
+            T* dst = reinterpret_cast<T*>(a.out) + b * a.o_b + t * a.o_t + (h * a.G + row0 + rr - t * a.G) * a.o_h + piece * 8;
+            if (vec) {
+              *reinterpret_cast<float4*>(dst) = f;
+            } else {
+              const T* e8 = reinterpret_cast<const T*>(&f);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) dst[e] = e8[e];
+            }
           }
         }
       }
-      __syncwarp();  // (the next load is the whole warp's)
     }
-    if (chunks > 1) {
-      if (in) *reinterpret_cast<float2*>(a.partial + a.partial_ml + at * 2) = make_float2(top_run, l);
-      // the last CTA of the chunks adds them up (below)
-      __threadfence();
-      named_bar_sync(1, 128 * NQ);
-      if (threadIdx.x == 128) *last_one = atomicAdd(a.tickets + ticket, 1u) == (uint32_t)chunks - 1;
-    }
+    if (partial && in) *reinterpret_cast<float2*>(a.partial + a.partial_ml + (at + r) * 2) = make_float2(top_run, l);
   } else if (warp >= 12) {
     // ------------------------------------------------------------------ codes to f16 tiles
     constexpr int CH = D / 16, UN = BN * CH / (32 * kConvert), TPI = 32 * kConvert / CH;  // chunks of a key, chunks a thread, keys apart
@@ -621,45 +634,68 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (chunks == 1 || !*last_one) return;
-  // All threads, in the order of the chunks: first every row's share of each, then the sums, several loads in flight.
-  __threadfence();
-  const int ticket = b * a.H * a.row_tiles + y;
-  if (threadIdx.x == 0) a.tickets[ticket] = 0;
-  const int64_t from = (int64_t)ticket * a.splits * L::ROWS;
+}
+
+// Adds the key ranges of a row tile up, in their order: a warp a row, all of a row's loads of eight ranges in flight.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) cache_attend_combine_kernel(const __grid_constant__ AttendArgs a, const int vec) {
+  constexpr int ROWS = Tiles<D>::ROWS, PL = D / 128 > 0 ? D / 128 : 1;  // four elements a lane and load
+  const int lane = threadIdx.x & 31, y = blockIdx.y, b = blockIdx.z;
+  const int h = y / a.row_tiles, row0 = (y - h * a.row_tiles) * ROWS, r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  grid_dependency_wait();
+  const int len = min(max(a.lens[b], 0), a.max_pages * a.P);
+  const int nq = a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
+  const int rows = min(ROWS, nq * a.G - row0);
+  const int prefix = a.prefix ? a.prefix[b] : 0;
+  const int last = row0 + rows - 1;
+  const int most = rows <= 0 ? 0 : max(0, a.causal ? min(len, max(len - nq + last / a.G + 1, prefix)) : len);
+  const int chunks = max(1, (most + a.chunk - 1) / a.chunk);
+  if (r >= rows || chunks == 1) return;   // (one range: written by its CTA)
+  const int64_t from = (int64_t)(b * a.H * a.row_tiles + y) * a.splits * ROWS + r;
   const float2* ml = reinterpret_cast<const float2*>(a.partial + a.partial_ml) + from;
   const float* po = a.partial + from * D;
-  float* share = reinterpret_cast<float*>(smem);  // [chunk][row]: the operands' shared memory is free
-  for (int r = threadIdx.x; r < rows; r += kThreads) {
-    float m = -INFINITY, l = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < chunks; ++s) m = fmaxf(m, __ldcg(ml + s * L::ROWS + r).x);
-#pragma unroll 4
-    for (int s = 0; s < chunks; ++s) {
-      const float2 x = __ldcg(ml + s * L::ROWS + r);
-      const float f = x.x == -INFINITY ? 1.0f : ex2_approx_ftz(x.x - m);
-      share[s * L::ROWS + r] = f;
-      l = fmaf(f, x.y, l);
+  const bool on = 4 * lane < D;
+  float m = -INFINITY, l = 0.0f;
+  for (int s = lane; s < chunks; s += 32) m = fmaxf(m, __ldcg(ml + (int64_t)s * ROWS).x);
+#pragma unroll
+  for (int z = 16; z > 0; z >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, z));
+  float4 o[PL] = {};
+#pragma unroll 1
+  for (int s0 = 0; s0 < chunks; s0 += 8) {
+    float4 u[8][PL];
+    float2 x[8];
+#pragma unroll
+    for (int z = 0; z < 8; ++z) {
+      if (s0 + z < chunks) {
+        x[z] = __ldcg(ml + (int64_t)(s0 + z) * ROWS);
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+          if (on) u[z][p] = __ldcg(reinterpret_cast<const float4*>(po + (int64_t)(s0 + z) * ROWS * D + 128 * p) + lane);
+      }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int s = 0; s < chunks; ++s) share[s * L::ROWS + r] *= inv;
+#pragma unroll
+    for (int z = 0; z < 8; ++z) {
+      if (s0 + z < chunks) {
+        const float f = x[z].x == -INFINITY ? 1.0f : ex2_approx_ftz(x[z].x - m);
+        l = fmaf(f, x[z].y, l);
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+          o[p].x = fmaf(f, u[z][p].x, o[p].x);
+          o[p].y = fmaf(f, u[z][p].y, o[p].y);
+          o[p].z = fmaf(f, u[z][p].z, o[p].z);
+          o[p].w = fmaf(f, u[z][p].w, o[p].w);
+        }
+      }
+    }
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
-    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int s = 0; s < chunks; ++s) {
-      const float f = share[s * L::ROWS + r];
-      const float4 u = __ldcg(reinterpret_cast<const float4*>(po + ((int64_t)s * L::ROWS + r) * D + d));
-      o.x = fmaf(f, u.x, o.x);
-      o.y = fmaf(f, u.y, o.y);
-      o.z = fmaf(f, u.z, o.z);
-      o.w = fmaf(f, u.w, o.w);
-    }
-    const int t = (row0 + r) / a.G, hq = h * a.G + (row0 + r) - t * a.G;
-    T* dst = reinterpret_cast<T*>(a.out) + b * a.o_b + t * a.o_t + hq * a.o_h + d;
-    const uint32_t w0 = pack_out<T>(o.x, o.y), w1 = pack_out<T>(o.z, o.w);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int t = (row0 + r) / a.G;
+  T* out = reinterpret_cast<T*>(a.out) + b * a.o_b + t * a.o_t + (h * a.G + row0 + r - t * a.G) * a.o_h;
+#pragma unroll
+  for (int p = 0; p < PL; ++p) {
+    if (!on) break;
+    const uint32_t w0 = pack_out<T>(o[p].x * inv, o[p].y * inv), w1 = pack_out<T>(o[p].z * inv, o[p].w * inv);
+    T* dst = out + 128 * p + 4 * lane;
     if (vec) {
       *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
     } else {
@@ -683,9 +719,12 @@ int launch_tiles(const AttendArgs& a, int vec, cudaStream_t s) {
     if (e != cudaSuccess) return (int)e;
     attr_set[dev] = true;
   }
-  const dim3 grid((unsigned)a.splits, (unsigned)(a.H * a.row_tiles), (unsigned)a.B);
-  const cudaError_t e = launch_dep(cache_attend_tiles_kernel<D, T, CAP, SLOPES>, grid, dim3(kThreads), Tiles<D>::kSmem, s, 1,
-                                   dependent_launch_for((int64_t)a.B * a.T), a, vec);
+  const bool dep = dependent_launch_for((int64_t)a.B * a.T);
+  const unsigned tiles = (unsigned)(a.H * a.row_tiles);
+  cudaError_t e = launch_dep(cache_attend_tiles_kernel<D, T, CAP, SLOPES>, dim3((unsigned)a.splits, tiles, (unsigned)a.B), dim3(kThreads),
+                             Tiles<D>::kSmem, s, 1, dep, a, vec);
+  if (e == cudaSuccess && a.splits > 1)
+    e = launch_dep(cache_attend_combine_kernel<D, T>, dim3((unsigned)Tiles<D>::ROWS / 8, tiles, (unsigned)a.B), dim3(256), 0, s, 1, dep, a, vec);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
