@@ -3,6 +3,7 @@
 //
 // Both are bound by memory: two (four, gated) bytes a value in, one code out, 4 / 128 bytes of scales.
 #include <cuda_runtime.h>
+#include <string.h>
 
 #include "../../include/iflb200.h"
 #include "launch.cuh"
@@ -67,52 +68,89 @@ struct BlockQuantArgs {
   int64_t qs_row, qs_block;
 };
 
-// Sixteen lanes take a block of 128 columns, eight values each.  The maximum is taken of the bits of |v|: they order
-// as the values do and put NaN on top, so that a block with a NaN gets the scale NaN.  Divisions are IEEE ones.
+// silu(g) * u for two elements, with ex2 and the reciprocal to an ulp or two.
+__device__ __forceinline__ void silu_mul2(float& g0, float& g1, float u0, float u1) {
+  float z0, z1;
+  unpack2(mul2(pack2(g0, g1), pack2(-1.4426950408889634f, -1.4426950408889634f)), z0, z1);
+  float d0, d1;
+  unpack2(add2(pack2(ex2_approx_ftz(z0), ex2_approx_ftz(z1)), pack2(1.0f, 1.0f)), d0, d1);
+  unpack2(mul2(mul2(pack2(g0, g1), pack2(rcp_approx_ftz(d0), rcp_approx_ftz(d1))), pack2(u0, u1)), g0, g1);
+}
+
+// Eight lanes take a block of 128 columns, twice eight neighbouring values each, so that every load and store of the eight
+// is one piece of memory.  The maximum is taken of the bits of |v|: they order as the values do and put NaN on top, so
+// that a block with a NaN gets the scale NaN.  Divisions are IEEE ones.
+//
+// B200, 816 x [16384 | 16384] bf16: 21.0 us with sixteen lanes a block and 64-bit index arithmetic, @@ like this (66 MB:
+// 10.3 at the copy rate); what is left is the activation, some 20 instructions a value.
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) block_quant_kernel(const BlockQuantArgs a) {
   grid_dependency_wait();
-  const int lane = threadIdx.x & 15;
-  const int64_t groups = (int64_t)a.M * a.blocks;
-  const int64_t g0 = ((int64_t)blockIdx.x * kQuantThreads + threadIdx.x) >> 4;
-  const int64_t step = (int64_t)gridDim.x * (kQuantThreads / 16);
-  // (whole warps stay in the loop: the exchange below is among sixteen lanes of a warp)
-  for (int64_t g = g0; g - (threadIdx.x >> 4 & 1) < groups; g += step) {
+  const int lane = threadIdx.x & 7;
+  const int groups = a.M * a.blocks, step = (int)gridDim.x * (kQuantThreads / 8);  // (checked on the host)
+  // (whole warps stay in the loop: the exchange below is among eight lanes of a warp)
+  for (int g = (int)blockIdx.x * (kQuantThreads / 8) + (threadIdx.x >> 3); g - (int)(threadIdx.x >> 3 & 3) < groups; g += step) {
     const bool in = g < groups;
-    const int m = in ? (int)(g / a.blocks) : 0, b = in ? (int)(g - (int64_t)m * a.blocks) : 0;
+    const int m = in ? (int)((unsigned)g / (unsigned)a.blocks) : 0, b = in ? g - m * a.blocks : 0;
     const int k = b * kQuantBlock + lane * 8;
-    const int valid = in ? min(8, max(0, a.K - k)) : 0;
-    float v[8] = {};
-    if (VEC ? valid == 8 : valid > 0) {
-      const T* row = reinterpret_cast<const T*>(a.x) + (int64_t)m * a.ld_x + k;
-      load_eight<VEC>(row, valid, v);
-      if (ACT >= 0) {
-        float u[8];
-        load_eight<VEC>(row + a.K, valid, u);
+    float v[2][8];
+    int valid[2];
+    const T* row = reinterpret_cast<const T*>(a.x) + (int64_t)m * a.ld_x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (ACT == IFLB200_ACT_SILU ? silu_ref(v[i]) : gelu_tanh_ref(v[i])) * u[i];
+    for (int z = 0; z < 2; ++z) {
+      valid[z] = in ? min(8, max(0, a.K - k - 64 * z)) : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[z][i] = 0.0f;
+      if (VEC ? valid[z] == 8 : valid[z] > 0) load_eight<VEC>(row + k + 64 * z, valid[z], v[z]);
+    }
+    if (ACT >= 0) {
+      float u[2][8];
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[z][i] = 0.0f;
+        if (VEC ? valid[z] == 8 : valid[z] > 0) load_eight<VEC>(row + a.K + k + 64 * z, valid[z], u[z]);
+      }
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          if (ACT == IFLB200_ACT_SILU) {
+            silu_mul2(v[z][i], v[z][i + 1], u[z][i], u[z][i + 1]);
+          } else {
+            gelu_tanh_ref2(v[z][i], v[z][i + 1]);
+            v[z][i] *= u[z][i];
+            v[z][i + 1] *= u[z][i + 1];
+          }
+        }
       }
     }
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i >> 3][i & 7]) & 0x7FFFFFFFu);
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    for (int d = 4; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
     const float amax = __uint_as_float(max(top, 0x322BCC77u));  // 1e-8
     const float inv = __fdiv_rn(448.0f, amax);
-    if (valid > 0) {
-      uint8_t* q = a.q + (int64_t)m * a.ld_q + k;
-      const uint32_t lo = cvt_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-      const uint32_t hi = cvt_e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-      if (VEC) {
-        *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
-      } else {
+    const uint64_t inv2 = pack2(inv, inv);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < valid) q[i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+    for (int z = 0; z < 2; ++z) {
+      if (valid[z] > 0) {
+        float c[8];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) unpack2(mul2(pack2(v[z][i], v[z][i + 1]), inv2), c[i], c[i + 1]);
+        uint8_t* q = a.q + (int64_t)m * a.ld_q + k + 64 * z;
+        const uint32_t lo = cvt_e4m3x4(c[0], c[1], c[2], c[3]), hi = cvt_e4m3x4(c[4], c[5], c[6], c[7]);
+        if (VEC) {
+          *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < valid[z]) q[i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+        }
       }
-      if (lane == 0) a.qs[m * a.qs_row + b * a.qs_block] = __fdiv_rn(amax, 448.0f);
     }
+    if (lane == 0 && in) a.qs[m * a.qs_row + b * a.qs_block] = __fdiv_rn(amax, 448.0f);
   }
   grid_launch_dependents();
 }
@@ -124,7 +162,7 @@ static int launch_block_quant(const BlockQuantArgs& a, cudaStream_t s) {
   const int64_t groups = (int64_t)a.M * a.blocks;
   const int sms = device_sm_count();
   if (sms == 0) return IFLB200_ERR_DEVICE;
-  const int64_t want = (groups + kQuantThreads / 16 - 1) / (kQuantThreads / 16), most = (int64_t)sms * 8;
+  const int64_t want = (groups + kQuantThreads / 8 - 1) / (kQuantThreads / 8), most = (int64_t)sms * 8;
   const dim3 grid((unsigned)(want < most ? want : most));
   const bool dep = dependent_launch_for(a.M);
   const cudaError_t e = vec ? launch_dep(block_quant_kernel<T, ACT, true>, grid, dim3(kQuantThreads), 0, s, 1, dep, a)
@@ -173,11 +211,32 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-template <typename T, bool VEC>
+// Eight values as they lie in memory.
+template <typename T>
+struct Piece {
+  uint4 w[sizeof(T) / 2];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* p) {
+    if (VEC) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      T x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = p[i];
+      memcpy(w, x, sizeof(w));
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const { load_eight<true>(reinterpret_cast<const T*>(w), 8, v); }
+};
+
+// Pieces stay in registers between the maximum and the codes, up to four a thread; a larger page reads the rest again.
+template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const AppendArgs a) {
+  constexpr int VECS = D / 8, KEEP = 4;
   grid_dependency_wait();
   const int b = blockIdx.z, h = blockIdx.y, which = blockIdx.x & 1, span = blockIdx.x >> 1;
-  const int P = a.page_tokens, D = a.head_dim;
+  const int P = a.page_tokens;
   const int64_t start = a.start[b];
   const int count = a.counts ? min(max(a.counts[b], 0), a.T) : a.T;
   if (start < 0) return;
@@ -185,48 +244,74 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const Appe
   const int lo = (int)max((int64_t)0, start - at), hi = (int)min((int64_t)P, start + count - at);
   if (lo >= hi || slot >= a.max_pages) return;
   const int page = a.table[b * a.ld_table + slot];
+  const T* src = reinterpret_cast<const T*>(a.src[which]) + b * a.sb[which] + (at - start + lo) * a.st[which] + h * a.sh[which];
+  const int64_t st = a.st[which];
+  const int n = (hi - lo) * VECS;
+  Piece<T> v[KEEP];
+  uint32_t top = 0;
+  auto highest = [&](const float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t bits = __float_as_uint(x[e]) & 0x7FFFFFFFu;
+      top = max(top, bits < 0x7F800000u ? bits : 0u);
+    }
+  };
+#pragma unroll
+  for (int z = 0; z < KEEP; ++z) {
+    const int i = threadIdx.x + z * blockDim.x;
+    if (i < n) v[z].template load<VEC>(src + (i / VECS) * st + i % VECS * 8);
+  }
   if (page < 0 || page >= a.pages) return;
   float* scale = a.scale[which] + (int64_t)page * a.heads + h;
   const float old = lo > 0 ? *scale : 0.0f;
-  const T* src = reinterpret_cast<const T*>(a.src[which]) + b * a.sb[which] + (at - start) * a.st[which] + h * a.sh[which];
-  const int64_t st = a.st[which];
-  const int vecs = D / 8, n = (hi - lo) * vecs;
-  uint32_t top = 0;
-  for (int i = threadIdx.x; i < n; i += kAppendThreads) {
-    float v[8];
-    const int j = lo + i / vecs;
-    load_eight<VEC>(src + j * st + (i - (i / vecs) * vecs) * 8, 8, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t bits = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-      top = max(top, bits < 0x7F800000u ? bits : 0u);
+  for (int z = 0; z < KEEP; ++z)
+    if ((int)(threadIdx.x + z * blockDim.x) < n) {
+      float x[8];
+      v[z].values(x);
+      highest(x);
     }
+  for (int i = threadIdx.x + KEEP * blockDim.x; i < n; i += blockDim.x) {
+    float x[8];
+    load_eight<VEC>(src + (i / VECS) * st + i % VECS * 8, 8, x);
+    highest(x);
   }
   __shared__ uint32_t tops[kAppendThreads / 32];
   top = __reduce_max_sync(0xFFFFFFFFu, top);
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) top = max(top, tops[w]);
+  if (blockDim.x > 32) {
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) top = max(top, tops[w]);
+  }
   const float now = fmaxf(old, page_scale(top));
   uint8_t* codes = a.codes[which] + ((int64_t)page * a.heads + h) * P * D;
   const bool two = (__float_as_uint(now) & 0x7FFFFFu) == 0;  // (a scale of another origin need not be a power of two)
   const float inv = __fdiv_rn(1.0f, now);
-  for (int i = threadIdx.x; i < n; i += kAppendThreads) {
-    float v[8];
-    const int j = lo + i / vecs, d = (i - (i / vecs) * vecs) * 8;
-    load_eight<VEC>(src + j * st + d, 8, v);
+  auto write = [&](int i, float (&x)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] = two ? v[e] * inv : __fdiv_rn(v[e], now);
-      if (fabsf(v[e]) > 3e38f) v[e] = __uint_as_float(0x7FC00000u);  // an infinity is no e4m3 value: NaN
+      x[e] = two ? x[e] * inv : __fdiv_rn(x[e], now);
+      if (fabsf(x[e]) > 3e38f) x[e] = __uint_as_float(0x7FC00000u);  // an infinity is no e4m3 value: NaN
     }
-    *reinterpret_cast<uint2*>(codes + j * D + d) =
-        make_uint2(cvt_e4m3x4(v[0], v[1], v[2], v[3]), cvt_e4m3x4(v[4], v[5], v[6], v[7]));
+    *reinterpret_cast<uint2*>(codes + lo * D + i * 8) = make_uint2(cvt_e4m3x4(x[0], x[1], x[2], x[3]), cvt_e4m3x4(x[4], x[5], x[6], x[7]));
+  };
+#pragma unroll
+  for (int z = 0; z < KEEP; ++z) {
+    const int i = threadIdx.x + z * blockDim.x;
+    if (i < n) {
+      float x[8];
+      v[z].values(x);
+      write(i, x);
+    }
+  }
+  for (int i = threadIdx.x + KEEP * blockDim.x; i < n; i += blockDim.x) {
+    float x[8];
+    load_eight<VEC>(src + (i / VECS) * st + i % VECS * 8, 8, x);
+    write(i, x);
   }
   if (lo > 0 && now > old) {
     const float ratio = __fdiv_rn(old, now);
-    for (int i = threadIdx.x; i < lo * vecs; i += kAppendThreads) {
+    for (int i = threadIdx.x; i < lo * VECS; i += blockDim.x) {
       uint2* at8 = reinterpret_cast<uint2*>(codes) + i;
       const uint2 u = *at8;
       const float2 p0 = e4m3x2_to_f32(u.x & 0xFFFF), p1 = e4m3x2_to_f32(u.x >> 16), p2 = e4m3x2_to_f32(u.y & 0xFFFF),
@@ -239,6 +324,12 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const Appe
   grid_launch_dependents();
 }
 
+template <typename T, int D>
+static cudaError_t launch_append(const AppendArgs& a, bool vec, const dim3& grid, int threads, bool dep, cudaStream_t s) {
+  return vec ? launch_dep(cache_append_kernel<T, D, true>, grid, dim3(threads), 0, s, 1, dep, a)
+             : launch_dep(cache_append_kernel<T, D, false>, grid, dim3(threads), 0, s, 1, dep, a);
+}
+
 template <typename T>
 static int launch_append(const AppendArgs& a, int B, cudaStream_t s) {
   uintptr_t bytes = 0;
@@ -246,9 +337,13 @@ static int launch_append(const AppendArgs& a, int B, cudaStream_t s) {
     bytes |= reinterpret_cast<uintptr_t>(a.src[i]) | (uintptr_t)((a.sb[i] | a.st[i] | a.sh[i]) * (int64_t)sizeof(T));
   const int64_t spans = ((int64_t)a.T + a.page_tokens - 2) / a.page_tokens + 1;
   const dim3 grid((unsigned)(2 * spans), (unsigned)a.heads, (unsigned)B);
-  const bool dep = dependent_launch_for((int64_t)B * a.T);
-  const cudaError_t e = bytes % 16 == 0 ? launch_dep(cache_append_kernel<T, true>, grid, dim3(kAppendThreads), 0, s, 1, dep, a)
-                                        : launch_dep(cache_append_kernel<T, false>, grid, dim3(kAppendThreads), 0, s, 1, dep, a);
+  const bool dep = dependent_launch_for((int64_t)B * a.T), vec = bytes % 16 == 0;
+  // as many threads as a page gets pieces of eight values; one warp needs no barrier
+  const int pieces = (a.T < a.page_tokens ? a.T : a.page_tokens) * a.head_dim / 8;
+  const int threads = pieces >= kAppendThreads ? kAppendThreads : (pieces + 31) / 32 * 32;
+  const cudaError_t e = a.head_dim == 64 ? launch_append<T, 64>(a, vec, grid, threads, dep, s)
+                                         : (a.head_dim == 128 ? launch_append<T, 128>(a, vec, grid, threads, dep, s)
+                                                              : launch_append<T, 256>(a, vec, grid, threads, dep, s));
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
@@ -262,7 +357,7 @@ extern "C" int iflb200_block_quant(const void* x, int x_dtype, int64_t ld_x, int
   if (act < -1 || act > IFLB200_ACT_SILU) return IFLB200_ERR_ARG;
   if (x_dtype != IFLB200_F32 && x_dtype != IFLB200_BF16 && x_dtype != IFLB200_F16) return IFLB200_ERR_DTYPE;
   if (M == 0 || K == 0) return IFLB200_OK;
-  if (K > (1 << 29)) return IFLB200_ERR_SHAPE;
+  if (K > (1 << 29) || (int64_t)M * ((K + kQuantBlock - 1) / kQuantBlock) > (1ll << 31) - (1 << 24)) return IFLB200_ERR_SHAPE;
   if (!x || !q || !qs) return IFLB200_ERR_ARG;
   if (ld_x < (int64_t)K * (act >= 0 ? 2 : 1) || ld_q < K || qs_row < 0 || qs_block < 0) return IFLB200_ERR_ARG;
   BlockQuantArgs a = {x, ld_x, M, K, (K + kQuantBlock - 1) / kQuantBlock, reinterpret_cast<uint8_t*>(q), ld_q, qs, qs_row, qs_block};

@@ -576,6 +576,49 @@ int operand_map(CUtensorMap* tm, const void* ptr, int rows, int K, int64_t ld, i
 // iflb200_block_linear_set_form; zeros: by rule
 int g_form = 0, g_tokens = 0, g_splits = 0;
 
+// Form, tokens of a tile and CTAs to a K range of least estimated time; what is given (not 0) stays.
+//
+// In microseconds, fitted to 22 shapes (1 to 4680 tokens, 1024 to 32768 columns, 512 to 16384 deep; every width and split of
+// each): a stage takes 0.30 + 0.0016 a token on single CTAs up to 64 tokens and 0.005 a token more above (both operands come
+// through one SM), 0.45 on pairs up to 64 tokens and 0.0025 a token more up to 0.575; a quarter less where the GPU is empty.
+// A tile's end is 0.4 + 0.006 a token.  Handing partial sums over is 0.4 + 0.25 a CTA; 33 clusters of four and 16 of eight fit
+// the GPU.  With it the chosen form was within 8 % of the fastest of all on those shapes.
+void choose(int M, int N, int stages, int out_dtype, int sms, int& form, int& bt, int& splits) {
+  const int staging = out_dtype == IFLB200_F32 ? 2048 : 1024;
+  const int form0 = form, bt0 = bt, splits0 = splits;
+  double best = 1e30;
+  int before = 0;
+  for (int t = bt0 ? bt0 : 16; t <= (bt0 ? bt0 : kAcc); t += 16) {
+    const int blocks = (M + t - 1) / t;
+    if (!bt0 && blocks == before) continue;  // no fewer tiles than the narrower ones
+    before = blocks;
+    const double end = 0.4 + 0.006 * t, over = t > 64 ? t - 64 : 0;
+    for (int f = form0 ? form0 : 1; f <= (form0 ? form0 : 2); ++f) {
+      for (int k = splits0 && f == 1 ? splits0 : 1; k <= (f == 2 ? 1 : (splits0 ? splits0 : 8)); k *= 2) {
+        if (k > 1 && (k > stages || Layout<1>::stages(t, k, staging) < 2)) continue;  // (a stage in flight needs a second beside it)
+        const int64_t units = (int64_t)blocks * ((N + f * kStep - 1) / (f * kStep)) * k;
+        const int64_t room = f == 2 ? sms / 2 : (k == 8 ? 128 : (k == 4 ? sms - 16 : sms));
+        const int64_t waves = (units + room - 1) / room;
+        if (k > 1 && waves > 1 && !splits0) continue;
+        const double load = waves == 1 ? (double)units / room : 1.0;
+        const double stage = (f == 1 ? 0.30 + 0.0016 * t + 0.0034 * over : (0.45 + 0.0025 * over < 0.575 ? 0.45 + 0.0025 * over : 0.575)) * (0.75 + 0.25 * load);
+        const double time = waves * ((stages + k - 1) / k * stage + end) + (k > 1 ? 0.4 + 0.25 * k : 0.0);
+        if (time < best) {
+          best = time;
+          form = f;
+          bt = t;
+          splits = k;
+        }
+      }
+    }
+  }
+  if (best == 1e30) {  // (only with a given split that does not fit)
+    form = form0 ? form0 : 1;
+    bt = bt0 ? bt0 : (M < kAcc ? (M + 15) / 16 * 16 : kAcc);
+    splits = 1;
+  }
+}
+
 template <int CG>
 int launch_form(const void* a, int64_t ld_a, const void* w, int64_t ld_w, BlockParams p, int bt, int splits, int sms, cudaStream_t s) {
   using L = Layout<CG>;
@@ -658,16 +701,7 @@ extern "C" int iflb200_block_linear(const void* a, int64_t ld_a, const void* w, 
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int steps = (K + SL * kStep - 1) / (SL * kStep);  // stages
   int form = g_form, bt = g_tokens, splits = g_splits;
-  if (form == 0) form = M <= 128 ? 1 : 2;
-  if (bt == 0) bt = M >= kAcc ? kAcc : (M + 15) / 16 * 16;
+  choose(M, N, steps, out_dtype, sms, form, bt, splits);
   if (form == 2) return launch_form<2>(a, ld_a, w, ld_w, p, bt, 1, sms, s);
-  const int64_t tiles = (int64_t)((M + bt - 1) / bt) * ((N + kStep - 1) / kStep);
-  if (splits == 0) {
-    splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= sms && steps >= splits * 2) splits *= 2;
-  }
-  // a stage that is refilled while its accumulator waits needs a second one beside it
-  const int staging = out_dtype == IFLB200_F32 ? 2048 : 1024;
-  while (splits > 1 && (splits > steps || Layout<1>::stages(bt, splits, staging) < 2)) splits /= 2;
   return launch_form<1>(a, ld_a, w, ld_w, p, bt, splits, sms, s);
 }
