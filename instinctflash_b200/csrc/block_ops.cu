@@ -81,7 +81,7 @@ __device__ __forceinline__ void silu_mul2(float& g0, float& g1, float u0, float 
 // is one piece of memory.  The maximum is taken of the bits of |v|: they order as the values do and put NaN on top, so
 // that a block with a NaN gets the scale NaN.  Divisions are IEEE ones.
 //
-// B200, 816 x [16384 | 16384] bf16: 21.0 us with sixteen lanes a block and 64-bit index arithmetic, @@ like this (66 MB:
+// B200, 816 x [16384 | 16384] bf16: 21.0 us with sixteen lanes a block and 64-bit index arithmetic, 13.7 us like this (66 MB:
 // 10.3 at the copy rate); what is left is the activation, some 20 instructions a value.
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) block_quant_kernel(const BlockQuantArgs a) {

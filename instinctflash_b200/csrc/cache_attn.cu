@@ -70,7 +70,7 @@ __device__ __forceinline__ void put4(T* p, float a, float b, float c, float d, i
 // codes) / l.  Sixteen tiles' pages and scales are looked up at a time, one unit of sixteen keys a lane.
 //
 // The code is kept short (loops over stages are not unrolled, what is rare is out of the way): a step of few rows is as much
-// instruction fetch as memory.  @@
+// instruction fetch as memory (32 sequences up to 8192 long, 8 heads of 128 with four rows each: 248 -> 80 us when it was made short).
 // ---------------------------------------------------------------------------------------------
 
 // NaN codes of a tile's values: the first key that has one, by column, and zeros in their place.
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
       if ((lane >> 1) == (tile & 15)) {
         // (a value scale of zero: the weights count, their product is nothing)
         const bool nil = vs == 0.0f;
-        unit[warp][stage][lane & 1] = make_float4(ks, nil ? 0.0f : log2_approx(vs), nil ? 1.0f : 1.0f / vs, page < 0 ? -1.0f : (nil ? 0.0f : 1.0f));
+        unit[warp][stage][lane & 1] = make_float4(ks, nil ? kNilLog2 : log2_approx(vs), nil ? kNilInverse : 1.0f / vs, page < 0 ? -1.0f : (nil ? 0.0f : 1.0f));
       }
       const int p0 = __shfl_sync(0xFFFFFFFFu, page, src), p1 = __shfl_sync(0xFFFFFFFFu, page, src + 1);
       const int i0 = __shfl_sync(0xFFFFFFFFu, in_page, src), i1 = __shfl_sync(0xFFFFFFFFu, in_page, src + 1);

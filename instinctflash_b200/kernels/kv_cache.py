@@ -131,7 +131,8 @@ def cache_attention(q: torch.Tensor, cache: KVCache8, table: torch.Tensor, lens:
     ``q_lens`` [B] int32: only the first ``q_lens[b]`` tokens of a row are there; the rows of ``out`` behind them are left
     as they were.  A query that sees no key gets zeros.  A length above what the table holds counts as what it holds;
     tokens of a page that is no page of the cache are masked.  Keys and values that a query does not see may hold
-    anything.  The value scales of one head's pages may lie within 2^60 of one another.
+    anything.  A value scale is 0 (the page's values are zeros) or lies between 2^-60 and 2^60.  ``out`` must not overlap
+    itself, nor ``q`` unless it is ``q``.
 
     ``workspace``: see ``attention_workspace``; without one a sequence is not shared among multiprocessors."""
     if native.cache_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, lens, out, causal, prefix, softcap,

@@ -241,6 +241,22 @@ def test_scales_far_apart_and_large_scores(T):
     check_attention(q * 3e4 if q.dtype == torch.bfloat16 else q, cache, table, lens, scale=1e-6)
 
 
+@pytest.mark.parametrize("T,D", [(1, 128), (5, 64), (2, 256), (90, 128), (90, 256)])
+def test_pages_with_a_value_scale_of_zero(T, D):
+    """Their keys count, their values are zeros (a NaN stays one), and the others' small values keep their bits."""
+    q, cache, table = scene(1, T, 4, 1, D, 16, 300)
+    used = table[0].long()
+    cache.v_scale[used, 0] = 2.0 ** -20
+    cache.v_scale[used[0::3], 0] = 0.0
+    check_attention(q, cache, table, ints(300), kv_cache.attention_workspace(DEV))
+    u8(cache.v)[used[3], 0, 2, 7] = 0x7F
+    u8(cache.v)[used[-1], 0, 9, 11] = 0xFF
+    cache.v_scale[used[-1], 0] = 0.0
+    check_attention(q, cache, table, ints(300))
+    cache.v_scale[used, 0] = 0.0
+    check_attention(q, cache, table, ints(299), kv_cache.attention_workspace(DEV))
+
+
 def test_wide_range_of_q_and_its_strides():
     q, cache, table = scene(2, 3, 8, 2, 128, 16, 100)
     lens = ints(100, 64)
