@@ -539,22 +539,32 @@ int launch_rows(const AttendArgs& a, cudaStream_t s) {
 
 // iflb200_cache_attention_set_form; 0: by rule
 int g_form = 0;
-constexpr int64_t kFewRows = 32;
 
+// Few rows take 16 rows (8 of 256 elements) at a time and are faster up to 64 rows of one head (32): row tiles cost the same
+// up to 256 (128) rows.  Few rows / tiles, 4 sequences of 16384 keys, 8 heads of 128: 63 / 118 us with 32 rows, 108 / 118 with
+// 64, 150 / 118 with 96; 16 of 4096, two heads of 256: 35 / 62 with 16, 66 / 64 with 32, 80 / 64 with 40.
 template <typename T>
 int attend(AttendArgs a, int D, void* workspace, int64_t bytes, cudaStream_t s) {
   const int64_t rows = (int64_t)a.T * a.G;
-  const bool many = g_form == 2 || (g_form == 0 && rows > kFewRows);
+  const bool many = g_form == 2 || (g_form == 0 && rows > (D == 256 ? 32 : 64));
   const int nt = D == 256 || rows <= 8 ? 1 : 2, per = many ? attend_tiles_rows(D) : 8 * nt;
   const int64_t tiles = (rows + per - 1) / per;
   if (tiles * a.H > 65535) return IFLB200_ERR_SHAPE;
   a.row_tiles = (int)tiles;
   const int sms = device_sm_count();
   if (sms == 0) return IFLB200_ERR_DEVICE;
-  // Chunks of keys: enough for some waves of CTAs, none shorter than a step of all warps, as many as the workspace takes.
+  // Ranges of keys, of whole steps of all warps, as many as the workspace takes and no more than fill the GPU once (few rows:
+  // as many CTAs an SM as share its issue slots without loss), where that is two or more.  Where it is not, sequences of
+  // different lengths are evened out: few rows over eight CTAs an SM, row tiles over two ranges while there are fewer than SMs.
+  //   16384 keys, 8 heads of 256, 8 rows, two sequences: 84.6 us with 74 ranges, 43.0 with 9, 86.0 with 2
+  //   32 sequences of 2048 to 8192 keys, 8 heads of 128, 4 rows: 67 us with five, 76 with three
+  //   the same of 1 to 8192 keys: 65 us with five, 59.4 with three, 77.8 unshared
+  //   row tiles, 16384 keys, 8 heads of 128, one sequence: 58.0 us with 19 (152 CTAs), 44.1 with 16
   const int64_t keys = (int64_t)a.max_pages * a.P, units = (int64_t)a.B * a.H * tiles;
   constexpr int64_t kLeast = kWarps * kTile;
-  const int64_t want = ((many ? 1ll : 8ll) * sms + units - 1) / units;
+  const int64_t fill = (many ? 1 : (D == 64 ? 3 : (D == 128 ? 2 : 1))) * (int64_t)sms / units;
+  const int64_t even = many ? (units < sms ? 2 : 1) : (8ll * sms + units - 1) / units;
+  const int64_t want = fill >= 2 ? fill : even;
   // The tickets have a place of their own whatever the geometry: they are zero between calls, partial results are not.
   // (Sequences are only shared where there are fewer units than CTAs wanted.)
   constexpr int64_t head = 4096;
@@ -563,8 +573,16 @@ int attend(AttendArgs a, int D, void* workspace, int64_t bytes, cudaStream_t s) 
   int64_t splits = units * 4 > head ? 1 : (want < room ? want : room);
   if (splits > 512) splits = 512;  // (shares of the chunks are worked out in shared memory)
   if (splits < 1) splits = 1;
-  int64_t chunk = ((keys + splits - 1) / splits + kLeast - 1) / kLeast * kLeast;
-  if (chunk < kLeast) chunk = kLeast;
+  const int64_t steps = (keys + kLeast - 1) / kLeast;
+  int64_t per_range = (steps + splits - 1) / splits;
+  if (per_range < 1) per_range = 1;
+  // The last CTA of few rows reads every range's result: five ranges cost about a step (16384 keys of one head of 256: 47 us
+  // with 128 ranges, 25.4 with 16 or 24, 51 with 4).
+  for (int64_t n = per_range + 1, best = 5 * per_range + (steps + per_range - 1) / per_range; !many && 5 * n < best; ++n) {
+    const int64_t cost = 5 * n + (steps + n - 1) / n;
+    if (cost < best) best = cost, per_range = n;
+  }
+  int64_t chunk = per_range * kLeast;
   if (chunk > (1 << 30)) chunk = 1 << 30;
   a.chunk = (int)chunk;
   a.splits = (int)((keys + chunk - 1) / chunk);
