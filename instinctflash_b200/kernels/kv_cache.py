@@ -98,8 +98,8 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, table: torch
     was: what the page holds below ``start[b]`` is rescaled where the scale grows (exactly, but for codes that fall below
     2^-6).  A page whose first token is written starts afresh.  Values that are not finite become NaN codes and do not
     enter the scale.  ``counts`` [B] int32: only the first ``counts[b]`` tokens of a row are there.  Tokens whose page lies
-    beyond the table, or whose entry is no page of the cache, are dropped.  A page must belong to one sequence of the call,
-    and what it holds at and above ``start[b] + counts[b]`` is not kept up."""
+    beyond the table, or whose entry is no page of the cache, are dropped, and so is a row with a negative start.  A page must
+    belong to one sequence of the call, and what it holds at and above ``start[b] + counts[b]`` is not kept up."""
     if native.cache_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, table, start, counts):
         return
     pages, heads, page_tokens, head_dim = _cache(cache)
@@ -132,7 +132,8 @@ def cache_attention(q: torch.Tensor, cache: KVCache8, table: torch.Tensor, lens:
     as they were.  A query that sees no key gets zeros.  A length above what the table holds counts as what it holds;
     tokens of a page that is no page of the cache are masked.  Keys and values that a query does not see may hold
     anything.  A value scale is 0 (the page's values are zeros) or lies between 2^-60 and 2^60.  ``out`` must not overlap
-    itself, nor ``q`` unless it is ``q``.
+    itself, nor ``q`` unless it is ``q``.  A table holds 2^30 tokens of a sequence at most, a call B up to 65535 and T * heads_q
+    up to eight million.
 
     ``workspace``: see ``attention_workspace``; without one a sequence is not shared among multiprocessors."""
     if native.cache_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, lens, out, causal, prefix, softcap,

@@ -95,6 +95,7 @@ def test_entry_points_reject_bad_arguments_before_any_launch():
                                            H, scale, cap, causal, p, 64, 64, 64, ws, wb, None)
     assert attend(B=0) == 0 and attend(T=0) == 0
     assert attend(HQ=3, H=2) == -2 and attend(D=80) == -2 and attend(P=8) == -2 and attend(mp=1 << 30) == -2
+    assert attend(T=1 << 28) == -2 and attend(T=1 << 30, HQ=4) == -2 and attend(B=1 << 16) == -2
     assert attend(dt=F32) == -4 and attend(q=None) == -1 and attend(lens=None) == -1 and attend(table=None) == -1
     assert attend(prefix=p, causal=0) == -1 and attend(cap=-1.0) == -1 and attend(cap=math.nan) == -1 and attend(scale=math.nan) == -1
     assert attend(ws=ctypes.c_void_p(4104), wb=8192) == -3 and attend(wb=-1) == -1

@@ -310,6 +310,67 @@ def test_offsets_beyond_32_bits():
     assert not cache.k[:-3].view(torch.uint8).any()
 
 
+@pytest.mark.parametrize("T", [1, 80])
+def test_empty_tables_caches_and_sequences(T):
+    q, cache, table = scene(2, T, 8, 2, 64, 16, 100)
+    ws = kv_cache.attention_workspace(DEV)
+    for c, t, lens in ((cache, table[:, :0], ints(50, 0)), (cache, table, ints(0, -3)),
+                       (kv_cache.KVCache8.empty(0, 2, 16, 64, DEV), table, ints(100, 7))):
+        for form in (1, 2, 0):
+            _lib.lib().iflb200_cache_attention_set_form(form)
+            out = torch.full_like(q, 7.5)
+            try:
+                kv_cache.cache_attention(q, c, t, lens, out, workspace=ws, causal=False)
+            finally:
+                _lib.lib().iflb200_cache_attention_set_form(0)
+            assert (out == 0).all()
+    k = torch.randn(2, T, 2, 64, device=DEV)
+    kv_cache.cache_append(kv_cache.KVCache8.empty(0, 2, 16, 64, DEV), k, k, table, ints(0, 0))
+    kv_cache.cache_append(cache, k, k, table[:, :0], ints(0, 0))
+
+
+@pytest.mark.parametrize("T,D", [(1, 128), (7, 256), (60, 128)])
+def test_output_over_q_and_the_same_bits_every_time(T, D):
+    q, cache, table = scene(3, T, 8, 2, D, 16, 1200)
+    lens, ws = ints(1200, 64, 700), kv_cache.attention_workspace(DEV)
+    first = kv_cache.cache_attention(q, cache, table, lens, torch.empty_like(q), workspace=ws)
+    for _ in range(5):
+        x = q.clone()
+        kv_cache.cache_attention(x, cache, table, lens, x, workspace=ws)
+        assert torch.equal(x, first)
+
+
+def test_two_streams_at_once_with_a_workspace_each():
+    scenes = [scene(1, t, 8, 2, 128, 16, 1500, seed=t) for t in (1, 40)]
+    lens = ints(1500)
+    ws = [kv_cache.attention_workspace(DEV) for _ in scenes]
+    want = [kv_cache.cache_attention(q, c, t, lens, torch.empty_like(q), workspace=w) for (q, c, t), w in zip(scenes, ws)]
+    outs = [torch.empty_like(q) for q, _, _ in scenes]
+    streams = [torch.cuda.Stream() for _ in scenes]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for (q, c, t), w, o, s in zip(scenes, ws, outs, streams):
+            with torch.cuda.stream(s):
+                kv_cache.cache_attention(q, c, t, lens, o, workspace=w)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, outs))
+
+
+def test_without_the_call_extension(monkeypatch):
+    """The same through ctypes."""
+    q, cache, table = scene(2, 3, 8, 2, 128, 16, 300)
+    twin = kv_cache.KVCache8(*(t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+    k = torch.randn(2, 3, 2, 128, device=DEV, generator=gen(1))
+    kw = dict(softcap=20.0, slopes=torch.rand(8, device=DEV), prefix=ints(5, 0), q_lens=ints(3, 2), workspace=kv_cache.attention_workspace(DEV))
+    outs = []
+    for c in (cache, twin):
+        kv_cache.cache_append(c, k, k, table, ints(90, 17), counts=ints(3, 1))
+        outs.append(kv_cache.cache_attention(q, c, table, ints(93, 18), torch.zeros_like(q), **kw))
+        for name in ("cache_append", "cache_attention"):
+            monkeypatch.setattr(kv_cache.native, name, lambda *a: False)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(u8(cache.k), u8(twin.k)) and torch.equal(cache.v_scale, twin.v_scale)
+
+
 def test_captured_steps_follow_lengths_and_share_a_workspace():
     """A decode step (append, attend) captured once and replayed as the sequences grow; a second graph with the same
     workspace in between."""
