@@ -354,9 +354,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
         const float now = exponents(i, v);
         high = fmaxf(high, now);
         if (__any_sync(0xFFFFFFFFu, now > 15.0f)) {
-          // more than that: all there is moves down, the weights of this step that are stored already too
+          // more than that: all there is moves down, the weights of this step that are stored already too (in fp32: they may be
+          // 2^15, and the factor less than f16 has)
           const float by = now > 15.0f ? ceilf(now) : 0.0f, f = ex2_approx_ftz(-by);
-          const uint32_t f2 = pack_half2(f, f);
           if (by > 0.0f) top_run += by;
           high = by > 0.0f ? 0.0f : high;
           l *= f;
@@ -371,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&w[e]), *reinterpret_cast<const __half2*>(&f2));
-              w[e] = *reinterpret_cast<const uint32_t*>(&x);
+              const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+              w[e] = pack_half2(p.x * f, p.y * f);
             }
             tmem_st_16(p_at + 16 * z, w);
           }

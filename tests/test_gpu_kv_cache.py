@@ -257,6 +257,27 @@ def test_pages_with_a_value_scale_of_zero(T, D):
     check_attention(q, cache, table, ints(299), kv_cache.attention_workspace(DEV))
 
 
+@pytest.mark.parametrize("low", [0.0, 6.0, 12.0, 14.0, 16.0, 20.0])
+@pytest.mark.parametrize("high", [16.0, 20.0, 26.0, 30.0, 60.0, 120.0])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scores_that_jump(D, low, high):
+    """Weights 2^0 on the first keys, then 2^low, then 2^high, each with values in columns of its own."""
+    q = torch.zeros(1, 2, 8, D, device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    cache = kv_cache.KVCache8.empty(20, 1, 16, D, DEV)
+    table = (torch.arange(16, device=DEV) + 2).to(torch.int32).view(1, 16)
+    k, v = torch.zeros(256, D, device=DEV), torch.zeros(256, D, device=DEV)
+    v[:128, 3] = 1.0
+    for at, exponent in ((130, low), (140, low), (170, high), (200, high - 9.0), (250, high)):
+        k[at, 0] = exponent
+        v[at, at % 64] = 448.0
+    for codes, x in ((cache.k, k), (cache.v, v)):
+        codes[2:18, 0] = x.view(16, 16, D).to(E4M3)
+    cache.k_scale.fill_(1.0)
+    cache.v_scale.fill_(1.0)
+    check_attention(q, cache, table, ints(256), scale=math.log(2.0), causal=False)
+
+
 def test_wide_range_of_q_and_its_strides():
     q, cache, table = scene(2, 3, 8, 2, 128, 16, 100)
     lens = ints(100, 64)
