@@ -62,11 +62,11 @@ __device__ __forceinline__ void put4(T* p, float a, float b, float c, float d, i
 // Keys on the MMA's M side, 8 rows on its N side.  Every warp walks key tiles of its own with a softmax state of its
 // own, loads (cp.async, one tile ahead, 16-byte pieces swizzled for ldmatrix) and all: no barrier until the end.
 // Codes become f16 in registers, which is exact; q is f16 too, its row brought near 1 by a power of two (a bf16 row keeps
-// all its bits down to 2^-14 of its largest element); weights are f16 relative to the row's running maximum.  All sums
+// all its bits down to 2^-14 of its largest element); weights are f16 with the row's running maximum at 2^10 (kWeightTop).  All sums
 // and the softmax state are fp32.
 //
 // The scales of a page are uniform over 16 keys: ks is part of the scores' factor, vs part of the exponent, as in
-// cache_attn_tiles.cu: weights 2^(y - M) with y = x + log2 vs, l = sum 2^(y - M) / vs, output = (sum of weights times
+// cache_attn_tiles.cu: weights 2^(y - M + 10) with y = x + log2 vs, l = sum 2^(y - M + 10) / vs, output = (sum of weights times
 // codes) / l.  Sixteen tiles' pages and scales are looked up at a time, one unit of sixteen keys a lane.
 //
 // The code is kept short (loops over stages are not unrolled, what is rare is out of the way): a step of few rows is as much
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
     uint32_t w[2][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float m[2] = {run[n][0] == -INFINITY ? 0.0f : run[n][0], run[n][1] == -INFINITY ? 0.0f : run[n][1]};
+      const float m[2] = {(run[n][0] == -INFINITY ? 0.0f : run[n][0]) - kWeightTop, (run[n][1] == -INFINITY ? 0.0f : run[n][1]) - kWeightTop};
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float p[4];

@@ -4,12 +4,12 @@
 //
 //   S = Q K^T            128 x BN x D, operands f16 in shared memory, S fp32 in tensor memory
 //   y = S * (factor of the row * ks) + log2 vs       base-2 exponents, masked at the edge
-//   P = 2^(y - M) as f16 into tensor memory          M: the row's running maximum of y
+//   P = 2^(y - M + 10) as f16 into tensor memory     M: the row's running maximum of y, 10: kWeightTop
 //   O += P V             128 x D x BN, P from tensor memory, V f16 in shared memory, O fp32 in tensor memory
 //
-// The value scale of a page is part of the exponent, so that O needs no scale of its own: with l = sum 2^(y - M) / vs
-// the output is O / l.  M moves only when a score passes it by more than 2^5, since O in tensor memory has to be
-// multiplied then.
+// The value scale of a page is part of the exponent, so that O needs no scale of its own: with l = sum 2^(y - M + 10) / vs
+// the output is O / l.  M moves only when a score passes it by more than 2^5, which is what f16 has room for, since O in tensor
+// memory has to be multiplied then.
 //
 // Codes become f16 on the way into shared memory (exact): a 16-bit operand of the same MMA rate as two 8-bit halves of q
 // and P would have, with 11 bits of P and no work on P but its rounding.  The MMA takes the values [key][D] as they lie
@@ -265,9 +265,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_at = tmem + lanes + kO + slot * D;
     float top_run = -INFINITY, l = 0.0f;
-    float drop = 1.0f;   // what O has yet to be multiplied by: a power of two
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
+      float drop = 1.0f;   // what O has to be multiplied by ahead of this step's product: a power of two
       const int buf = NQ == 2 ? slot : j & 1;
       const uint32_t phase = NQ == 2 ? j & 1u : (j >> 1) & 1u;
       const uint32_t s_at = tmem + lanes + kS + buf * BN, p_at = tmem + lanes + L::kP + buf * L::kPStride;
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
         m0 = lds_f4(m_at + 32 * i);
         m1 = lds_f4(m_at + 32 * i + 16);
         const float f0 = factor * m0.x * (CAP ? 1.0f : kLog2e), f1 = factor * m1.x * (CAP ? 1.0f : kLog2e);
-        const float base = top_run == -INFINITY ? 0.0f : top_run, c0 = m0.y - base, c1 = m1.y - base;
+        const float base = (top_run == -INFINITY ? 0.0f : top_run) - kWeightTop, c0 = m0.y - base, c1 = m1.y - base;
         tmem_ld_wait();
         if (CAP) {
 #pragma unroll
@@ -347,10 +347,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
           uint32_t v[32];
           first = fmaxf(first, exponents(i, v));
         }
-        if (none) top_run = first;
+        if (none) top_run = first - kWeightTop;
       }
-      // The weights, relative to the maximum of the steps before: f16 has room for 2^15 of it.
-      float high = -INFINITY;
+      // The weights, relative to the maximum of the steps before.
 #pragma unroll 1
       for (int i = 0; i < BN / 32; ++i) {
         uint32_t v[32];
@@ -365,13 +364,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
             t[e >> 4] = add2(t[e >> 4], pack2(p0, p1));
             w[e / 2] = pack_half2(p0, p1);
           }
-          if (__builtin_expect(!__any_sync(0xFFFFFFFFu, now > 15.0f), 1)) break;
-          // more than f16 has: all there is moves down, the weights of this step that are stored already too (in fp32: f16 may not
-          // have the factor)
-          const float by = now > 15.0f ? ceilf(now) : 0.0f, f = ex2_approx_ftz(-by);
+          if (__builtin_expect(!__any_sync(0xFFFFFFFFu, now > kWeightTop + kLazy), 1)) break;
+          // more than f16 has: the maximum moves by a whole power of two, and all there is down, the weights of this step that are
+          // stored already too (in fp32: f16 may not have the factor)
+          const float by = now > kWeightTop + kLazy ? ceilf(now - kWeightTop) : 0.0f, f = ex2_approx_ftz(-by);
           if (by > 0.0f) top_run += by;
-          high = by > 0.0f ? 0.0f : high;
-          now = by > 0.0f ? 0.0f : now;
+          now -= by;
           l *= f;
           drop *= f;
 #pragma unroll
@@ -390,7 +388,6 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
             tmem_st_16(p_at + 16 * z, u);
           }
         }
-        high = fmaxf(high, now);
         float t0, t1;
         unpack2(t[0], t0, t1);
         l = fmaf(t0 + t1, m0.z, l);
@@ -405,20 +402,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(PFULL, buf));
-      // the maximum moves when a score has passed it by more than kLazy, by a whole power of two; O follows at the next step
-      if (__any_sync(0xFFFFFFFFu, high > kLazy)) {
-        const float by = high > kLazy ? ceilf(high) : 0.0f, f = ex2_approx_ftz(-by);
-        if (by > 0.0f) top_run += by;
-        l *= f;
-        drop = f;
-      }
     }
     if (ok && steps > 0) ok = wait_warp(bar(PV, slot), (steps - 1) & 1u, abort_flag, (1u << 24) | (3u << 16));
     tc_fence_after();
     // The output through shared memory (this row tile of q is done with), 2 D bytes of each row at a time: whole rows go to
     // memory, where a row a thread would write half sectors.
     const bool any_nan = *nan_any != 0, partial = chunks > 1;
-    const float inv = drop * (partial ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l));  // (the last move of the maximum is still to be made)
+    const float inv = partial ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
     const uint32_t stage = q_at + slot * L::kQ + (warp & 3) * 32 * 2 * D;
     const int64_t at = ((int64_t)(b * a.H * a.row_tiles + y) * a.splits + split) * L::ROWS;
     constexpr int PR = D / 8;  // 16-byte pieces of a row

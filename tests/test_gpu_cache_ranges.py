@@ -1,0 +1,111 @@
+"""Attention over the 8-bit cache where weights, value scales, queries or positions cover a wide range: every key's share of the
+result within the error that the kernels' arithmetic leaves it, not only the largest ones'."""
+import math
+
+import pytest
+import torch
+
+from instinctflash_b200 import _lib
+from instinctflash_b200.kernels import kv_cache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+E4M3 = torch.float8_e4m3fn
+FORMS = (1, 2, 0)
+
+
+def ints(*v):
+    return torch.tensor(v, device=DEV, dtype=torch.int32)
+
+
+def cache_of(k, v, ks, vs, page, order=None):
+    """A cache of one sequence from rows [keys, heads, D] and scales [pages, heads]; its pages lie in ``order``."""
+    n, H, D = k.shape
+    pages = n // page
+    order = torch.arange(pages, device=DEV) if order is None else order
+    cache = kv_cache.KVCache8.empty(pages, H, page, D, DEV)
+    for codes, x in ((cache.k, k), (cache.v, v)):
+        codes[order] = x.view(pages, page, H, D).transpose(1, 2).to(E4M3)
+    cache.k_scale[order], cache.v_scale[order] = ks, vs
+    return cache, order.to(torch.int32).view(1, pages)
+
+
+def plain(q, cache, table, n, scale, flush, causal=True, slopes=None, first=0):
+    """Result in 64 bits for one sequence of ``n`` keys (those ahead of ``first`` have no weight), and the error allowed: scores in
+    fp32, weights as f16 (half a step, 2^-11 of each, or ``flush`` of the row's largest below f16's normal range), one rounding of the
+    result."""
+    T, HQ, D = q.shape[1:]
+    H, P = cache.k.shape[1:3]
+    j = torch.arange(first, n, device=DEV)
+    page = table[0].long()[j // P]
+    p = torch.arange(n - T, n, device=DEV)
+    out, tol = torch.zeros(T, HQ, D, device=DEV, dtype=torch.float64), torch.zeros(T, HQ, D, device=DEV, dtype=torch.float64)
+    for i in range(HQ):
+        h = i * H // HQ
+        key = cache.k[page, h, j % P].double() * cache.k_scale[page, h].double()[:, None]
+        val = cache.v[page, h, j % P].double() * cache.v_scale[page, h].double()[:, None]
+        x = q[0, :, i].double()
+        s, mag = x @ key.t() * scale, x.abs() @ key.abs().t() * abs(scale)
+        err = mag * (D + 8) * 2.0 ** -24
+        if slopes is not None:
+            bias = slopes[i].double() * (p[:, None] - j).abs()
+            s, err = s - bias, err + bias * 2.0 ** -22
+        err = err + s.abs() * 2.0 ** -22 + 2.0 ** -21     # to base 2, less the maximum, ex2
+        if causal:
+            s = s.masked_fill(j[None] > p[:, None], -math.inf)
+        w = torch.softmax(s, 1)
+        err = torch.where(w > 0, err, 0.0)
+        o = w @ val
+        share = torch.where(w > 0, w * (2.0 ** -11 + 2 * err) + flush * w.amax(1, keepdim=True), 0.0)
+        f16 = 2.0 ** -25 if q.dtype == torch.float16 else 0.0          # half of its least step
+        out[:, i] = o
+        tol[:, i] = share @ val.abs() + (w * 2 * err).sum(1, keepdim=True) * o.abs() + torch.finfo(q.dtype).eps / 2 * o.abs() + f16
+    return out, tol
+
+
+def check(q, cache, table, n, scale, flush, workspaces=(0, 16 << 20), forms=FORMS, **kw):
+    first = kw.pop("first", 0)
+    want, tol = plain(q, cache, table, n, scale, flush, first=first, **kw)
+    for nbytes in workspaces:
+        for form in forms:
+            out = torch.full_like(q, math.nan)
+            assert _lib.lib().iflb200_cache_attention_set_form(form) == 0
+            try:
+                kv_cache.cache_attention(q, cache, table, ints(n), out, scale=scale,
+                                         workspace=kv_cache.attention_workspace(DEV, nbytes) if nbytes else None, **kw)
+            finally:
+                _lib.lib().iflb200_cache_attention_set_form(0)
+            got = out[0].double()
+            assert torch.equal(got.isnan(), want.isnan()), f"form {form}, workspace {nbytes}: NaN in other places"
+            off = ((got - want).abs() - tol).nan_to_num(-1.0)
+            assert off.max() <= 0, f"form {form}, workspace {nbytes}: {float(off.max())} outside at {(off > 0).nonzero()[0].tolist()}"
+
+
+def rows_of(D, T=1, heads=4, dtype=torch.bfloat16):
+    """Queries that take columns 0 and 1 of the keys as they are: scores to base 2 with a scale of log 2."""
+    q = torch.zeros(1, T, heads, D, device=DEV, dtype=dtype)
+    q[..., :2] = 1.0
+    return q
+
+
+# A weight keeps f16's eleven bits down to 2^-24 of the row's largest (normal f16 with the largest at 2^10) and half a step of f16's
+# subnormals, 2^-25 / 2^10, below; twice that where a step's weights move to a larger maximum after they were rounded.
+FLUSH = 2.0 ** -34
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("place", [0, 2000, 4095])
+@pytest.mark.parametrize("depth", [12.0, 18.0, 22.0, 24.0, 26.0, 28.0])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_long_tail_of_small_weights(D, depth, place, dtype):
+    """One key with nearly all the weight and no value in the tail's columns, 4095 keys 2^-depth below it that alone have some."""
+    n, g = 4096, torch.Generator(device=DEV).manual_seed(int(depth))
+    k, v = torch.zeros(n, 1, D, device=DEV), torch.zeros(n, 1, D, device=DEV)
+    k[:, 0, 1] = torch.randint(-11, 1, (n,), device=DEV, generator=g) / 16.0
+    v[:, 0, 2:34] = torch.rand(n, 32, device=DEV, generator=g) * 300.0 + 100.0
+    v[:, 0, 34:] = torch.randn(n, D - 34, device=DEV, generator=g) * 100.0
+    k[place], v[place] = 0.0, 0.0
+    k[place, 0, 0], v[place, 0, 1] = depth, 448.0
+    lift = torch.full((n // 64, 1), 2.0 ** 6, device=DEV)
+    cache, table = cache_of(k, v, torch.ones_like(lift), lift, 64)
+    check(rows_of(D, dtype=dtype), cache, table, n, math.log(2.0), FLUSH)
