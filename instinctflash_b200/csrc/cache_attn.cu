@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
 
   float acc[NT][CH][4] = {};  // output, transposed: elements 16 i + 2 g (c0, c1) and + 1 (c2, c3) of rows 2 c, 2 c + 1
   float run[NT][2], sum[NT][2];
+  float top_scale = -INFINITY;  // the largest value scale so far, to base 2
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -350,37 +351,91 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
     }
     // weights, 16 keys x 8 rows transposed into the MMA's B fragments, and their product with the codes
     uint32_t w[2][NT][2];
+    auto weights = [&](int u, int n, float m0, float m1, float inverse0, float inverse1) {
+      float p[4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float m[2] = {(run[n][0] == -INFINITY ? 0.0f : run[n][0]) - kWeightTop, (run[n][1] == -INFINITY ? 0.0f : run[n][1]) - kWeightTop};
+      for (int e = 0; e < 4; ++e) {
+        p[e] = ex2_approx_ftz(sc[u][n][e] - (e & 1 ? m1 : m0));
+        sum[n][e & 1] = fmaf(p[e], e & 1 ? inverse1 : inverse0, sum[n][e & 1]);
+      }
+      const bool nil = un[u].w == 0.0f;
+      w[u][n][0] = transpose8x8(nil ? 0u : pack_half2(p[0], p[1]));
+      w[u][n][1] = transpose8x8(nil ? 0u : pack_half2(p[2], p[3]));
+    };
+    // Values 16 i .. + 31 of a unit's keys as A fragments.
+    auto values = [&](int u, int i, uint32_t (&f)[2][4]) {
+      uint32_t r[4];
+      const int row = 16 * u + (lane & 15), chunk = i + (lane >> 4), sw = D == 64 ? chunk ^ (row >> 1 & 3) : chunk ^ (row & 7);
+      ldsm_x4_trans(vt + row * D + sw * 16, r);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        // a register has two elements of two neighbouring keys: pair the keys
+        const uint32_t lo = __byte_perm(r[2 * x], 0, 0x3120), hi = __byte_perm(r[2 * x + 1], 0, 0x3120);
+        f[x][0] = e4m3x2_f16x2(lo);
+        f[x][1] = e4m3x2_f16x2(lo >> 16);
+        f[x][2] = e4m3x2_f16x2(hi);
+        f[x][3] = e4m3x2_f16x2(hi >> 16);
+      }
+    };
+    const float scale0 = un[0].w > 0.0f ? un[0].y : INFINITY, scale1 = un[1].w > 0.0f ? un[1].y : INFINITY;
+    if (scale0 < INFINITY) top_scale = fmaxf(top_scale, scale0);
+    if (scale1 < INFINITY) top_scale = fmaxf(top_scale, scale1);
+    if (__builtin_expect(fminf(scale0, scale1) >= top_scale - kFar, 1)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float m0 = (run[n][0] == -INFINITY ? 0.0f : run[n][0]) - kWeightTop, m1 = (run[n][1] == -INFINITY ? 0.0f : run[n][1]) - kWeightTop;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) weights(u, n, m0, m1, un[u].z, un[u].z);
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = ex2_approx_ftz(sc[u][n][e] - m[e & 1]);
-          sum[n][e & 1] = fmaf(p[e], un[u].z, sum[n][e & 1]);
+        for (int i = 0; i < CH; i += 2) {
+          uint32_t f[2][4];
+          values(u, i, f);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(acc[n][i + x], f[x], w[u][n][0], w[u][n][1]);
         }
-        const bool nil = un[u].w == 0.0f;
-        w[u][n][0] = transpose8x8(nil ? 0u : pack_half2(p[0], p[1]));
-        w[u][n][1] = transpose8x8(nil ? 0u : pack_half2(p[2], p[3]));
       }
-    }
+    } else {
+      // a scale far below another: every unit's and row's largest weight moves to 2^10, and the product back by as much
+      float back[2][NT][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = 16 * u + (lane & 15);
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-      for (int i = 0; i < CH; i += 2) {
-        uint32_t r[4];
-        const int chunk = i + (lane >> 4), sw = D == 64 ? chunk ^ (row >> 1 & 3) : chunk ^ (row & 7);
-        ldsm_x4_trans(vt + row * D + sw * 16, r);
+        for (int n = 0; n < NT; ++n) {
+          float m[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          // a register has two elements of two neighbouring keys: pair the keys
-          const uint32_t lo = __byte_perm(r[2 * x], 0, 0x3120), hi = __byte_perm(r[2 * x + 1], 0, 0x3120);
-          const uint32_t f[4] = {e4m3x2_f16x2(lo), e4m3x2_f16x2(lo >> 16), e4m3x2_f16x2(hi), e4m3x2_f16x2(hi >> 16)};
+          for (int e = 0; e < 2; ++e) {
+            float t = fmaxf(sc[u][n][e], sc[u][n][e + 2]);
+            t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 4));
+            t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 8));
+            t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 16));
+            const float lift = t == -INFINITY ? 0.0f : fminf(floorf(run[n][e] - t), 120.0f);
+            m[e] = (run[n][e] == -INFINITY ? 0.0f : run[n][e]) - kWeightTop - lift;
+            back[u][n][e] = ex2_approx_ftz(-lift);
+          }
+          weights(u, n, m[0], m[1], un[u].z * back[u][n][0], un[u].z * back[u][n][1]);
+        }
+      }
+#pragma unroll 1
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(acc[n][i + x], f, w[u][n][0], w[u][n][1]);
+        for (int i = 0; i < CH; i += 2) {
+          uint32_t f[2][4];
+          values(u, i, f);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma_f16(t, f[x], u ? w[1][n][0] : w[0][n][0], u ? w[1][n][1] : w[0][n][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[n][i + x][e] = fmaf(t[e], u ? back[1][n][e & 1] : back[0][n][e & 1], acc[n][i + x][e]);
+            }
+          }
         }
       }
     }

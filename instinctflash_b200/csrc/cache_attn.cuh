@@ -32,14 +32,18 @@ struct AttendArgs {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
-// The value scale is part of the exponent (value scales of 2^-60 to 2^60 keep every weight that matters normal).  A scale of
-// zero counts as the smallest there, so that its weights, whose values are zeros, take no bits from others'.
+// The value scale is part of the exponent.  A scale of zero counts as 2^-60 there, so that its weights, whose values are zeros, take
+// no bits from others'.
 constexpr float kNilLog2 = -60.0f, kNilInverse = 1152921504606846976.0f;
 // Weights enter the product as f16.  The running maximum's is 2^10: a weight keeps eleven bits down to 2^-24 of it and half a step of
-// f16's subnormals, 2^-35 of it, below (with the
-// maximum at 1 a tail of 2^-22 came out wrong in its third digit, one of 2^-26 was lost).
+// f16's subnormals, 2^-35 of it, below (with the maximum at 1 a tail of 2^-22 came out wrong in its third digit, one of 2^-26 was
+// lost).  A page with a large value scale would take these bits from the other pages', which still are all there is in columns where
+// it has zeros.  So units whose scale is more than 2^6 below the largest one so far get weights with a maximum of their own (few
+// rows), or a pass over the keys for each 2^6 of scales, from the lowest up (row tiles): no weight is off by more than 2^-11 of it or
+// 2^-29 of its row's largest probability, whatever the scales.
 constexpr float kWeightTop = 10.0f;
 constexpr float kLazy = 5.0f;  // base-2 exponent by which a score may pass the running maximum before it moves: to 2^15
+constexpr float kFar = 6.0f;
 
 // cap * tanh(s / cap).  tanh(x) = 1 - 2 / (1 + e^2x) is off by 1e-7 of 1; near zero, where that is more than fp32 keeps
 // of the result, the series (next term below 1e-7 of x at 1/4).

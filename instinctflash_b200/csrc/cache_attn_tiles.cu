@@ -45,7 +45,7 @@ struct Tiles {
   static constexpr int kOff = kNan + D * 4 + 16;          // each converter warp's units of two steps: offset of the codes
   static constexpr int kHole = kOff + kConvert * 2 * GR * 8;  // of four steps: whether a unit has no page
   static constexpr int kFactor = kHole + 16;              // of each row of q
-  static constexpr int kBar = kFactor + ROWS * 4;
+  static constexpr int kBar = kFactor + ROWS * 4;         // barriers, address of the tensor memory, abort, bands of value scales
   static constexpr int kSmem = kBar + 24 * 8 + 16 + 1024;
 };
 
@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   auto bar = [&](int kind, int i) { return bar0 + 8u * (kind + i); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kBar + 24 * 8);
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  volatile uint32_t* far_bands = tmem_slot + 2;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // (the last row tiles first: under a causal mask they have the most keys)
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   // it moved at every step: 2048 tokens behind 6144, 32 heads, 507 us, 420 like this).
   auto key_of = [&](int step) { return key0 + (steps - 1 - step) * BN; };
 
-  if (threadIdx.x == 0) {
+  auto start_barriers = [&]() {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(KFULL, i), kConvert);
       mbar_init(bar(KEMPTY, i), 1);
@@ -185,8 +186,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
       mbar_init(bar(PFULL, i), 4);
       mbar_init(bar(PV, i), 1);
     }
+  };
+  if (threadIdx.x == 0) {
+    start_barriers();
     mbar_init(bar(QFULL, 0), 8);
     tmem_slot[1] = 0;
+    *far_bands = 0;
     *nan_any = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -201,6 +206,32 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+
+  // Passes over the keys.  The first one takes all; where it found value scales more than 2^kFar apart it is forgotten, and there is
+  // one for each band of 2^kFar that has a scale, from the lowest up, into the same sums (see kWeightTop).  Between passes no MMA and
+  // no arrival is on its way: the last product has been waited for, and a slot is only given back where a later step waits for it.
+  // 2048 tokens behind 6144, 32 heads: 395 us, 1245 with a third of the pages 2^8 or 2^27 below the rest (three passes); few rows
+  // lose 2 % by it (32 sequences of up to 8192 keys, one token: 88 and 90 us).
+  int band = -1;            // of value scales; -1: all
+  uint32_t bands = 0;       // that are still to come
+  auto band_of = [](float log2_scale) { return min(max((int)floorf((log2_scale + 96.0f) * (1.0f / kFar)), 0), 31); };
+  auto next_pass = [&]() {  // every warp, converged; the same answer for all
+    tc_fence_before();
+    named_bar_sync(2, kThreads);
+    if (band < 0) bands = *far_bands;
+    if (bands == 0 || *abort_flag) return false;
+    band = __ffs(bands) - 1;
+    bands &= bands - 1;
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < QFULL; ++i) mbar_inval(bar(i, 0));
+      start_barriers();
+      fence_barrier_init();
+      fence_proxy_async_smem();
+    }
+    named_bar_sync(2, kThreads);
+    tc_fence_after();
+    return true;
+  };
 
   if (warp >= 4 && warp < 12) {
     // The rows of q as f16, each row's largest element near 1: eight warps, LR lanes a row, eight loads in flight.
@@ -265,145 +296,150 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_at = tmem + lanes + kO + slot * D;
     float top_run = -INFINITY, l = 0.0f;
-    bool ok = true;
-    for (int j = 0; j < steps; ++j) {
-      float drop = 1.0f;   // what O has to be multiplied by ahead of this step's product: a power of two
-      const int buf = NQ == 2 ? slot : j & 1;
-      const uint32_t phase = NQ == 2 ? j & 1u : (j >> 1) & 1u;
-      const uint32_t s_at = tmem + lanes + kS + buf * BN, p_at = tmem + lanes + L::kP + buf * L::kPStride;
-      ok = wait_warp(bar(SFULL, buf), phase, abort_flag, (1u << 24) | (1u << 16) | (j & 0xFFFF));
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t m_at = meta + (j & 3) * GR * 16;  // of each unit: ks, log2 vs, 1 / vs, 0 where there is no page
-      const int key = key_of(j);
-      const bool edge = key + BN > least || *reinterpret_cast<volatile int*>(smem + L::kHole + (j & 3) * 4) != 0;
-      float4 m0, m1;
-      // Exponents of 32 columns (two units).  Everything here is a loop over 32 columns that is not unrolled: the parts of this
-      // kernel that run at the same time have to fit the instruction cache together.  With 128 columns unrolled an MMA was
-      // issued every 300 clocks (2048 tokens behind 6144, 32 heads: 746 us then; 495 like this).
-      auto exponents = [&](int i, uint32_t (&v)[32]) {
-        tmem_ld_32x32b_x32(s_at + 32 * i, v);
-        m0 = lds_f4(m_at + 32 * i);
-        m1 = lds_f4(m_at + 32 * i + 16);
-        const float f0 = factor * m0.x * (CAP ? 1.0f : kLog2e), f1 = factor * m1.x * (CAP ? 1.0f : kLog2e);
-        const float base = (top_run == -INFINITY ? 0.0f : top_run) - kWeightTop, c0 = m0.y - base, c1 = m1.y - base;
-        tmem_ld_wait();
-        if (CAP) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            v[e] = __float_as_uint(fmaf(soft_cap(__uint_as_float(v[e]) * (e < 16 ? f0 : f1), a.cap, inv_cap), kLog2e, e < 16 ? c0 : c1));
-        } else {
-          const uint64_t f[2] = {pack2(f0, f0), pack2(f1, f1)}, c[2] = {pack2(c0, c0), pack2(c1, c1)};
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float p0, p1;
-            unpack2(fma2(pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f[e >> 4], c[e >> 4]), p0, p1);
-            v[e] = __float_as_uint(p0);
-            v[e + 1] = __float_as_uint(p1);
-          }
-        }
-        if (SLOPES) {
-          const float from = pos - (float)(key + 32 * i);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fmaf(-slope, fabsf(from - (float)e), __uint_as_float(v[e])));
-        }
-        if (edge) {
-          const int n = limit - key - 32 * i, n0 = m0.w == 0.0f ? 0 : n, n1 = m1.w == 0.0f ? 0 : n;
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (e >= (e < 16 ? n0 : n1)) v[e] = 0xFF800000u;
-        }
-        float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) high[e >> 1 & 3] = max3(high[e >> 1 & 3], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-        return fmaxf(max3(high[0], high[1], high[2]), high[3]);
-      };
-      // O may change once the product of the step before is complete, and every phase of its barrier is waited for in turn.
-      auto settle = [&]() {
-        if (j > 0) ok = wait_warp(bar(PV, slot), (j - 1) & 1u, abort_flag, (1u << 24) | (2u << 16) | (j & 0xFFFF));
+    bool ok = true, fresh = true;  // fresh: nothing in O yet
+    for (;;) {
+      for (int j = 0; j < steps; ++j) {
+        float drop = 1.0f;   // what O has to be multiplied by ahead of this step's product: a power of two
+        const int buf = NQ == 2 ? slot : j & 1;
+        const uint32_t phase = NQ == 2 ? j & 1u : (j >> 1) & 1u;
+        const uint32_t s_at = tmem + lanes + kS + buf * BN, p_at = tmem + lanes + L::kP + buf * L::kPStride;
+        ok = wait_warp(bar(SFULL, buf), phase, abort_flag, (1u << 24) | (1u << 16) | (j & 0xFFFF));
+        if (!ok) break;
         tc_fence_after();
-        if (ok && __any_sync(0xFFFFFFFFu, drop != 1.0f)) {
-          if (j > 0) {
-#pragma unroll 1
-            for (int i = 0; i < D / 16; ++i) {
-              uint32_t o[16];
-              tmem_ld_16c(o_at + 16 * i, o);
-              tmem_ld_wait();
+        const uint32_t m_at = meta + (j & 3) * GR * 16;  // of each unit: ks, log2 vs, 1 / vs, 0 where there is no page
+        const int key = key_of(j);
+        const bool edge = key + BN > least || *reinterpret_cast<volatile int*>(smem + L::kHole + (j & 3) * 4) != 0;
+        float4 m0, m1;
+        // Exponents of 32 columns (two units).  Everything here is a loop over 32 columns that is not unrolled: the parts of this
+        // kernel that run at the same time have to fit the instruction cache together.  With 128 columns unrolled an MMA was
+        // issued every 300 clocks (2048 tokens behind 6144, 32 heads: 746 us then; 495 like this).
+        auto exponents = [&](int i, uint32_t (&v)[32]) {
+          tmem_ld_32x32b_x32(s_at + 32 * i, v);
+          m0 = lds_f4(m_at + 32 * i);
+          m1 = lds_f4(m_at + 32 * i + 16);
+          const float f0 = factor * m0.x * (CAP ? 1.0f : kLog2e), f1 = factor * m1.x * (CAP ? 1.0f : kLog2e);
+          const float base = (top_run == -INFINITY ? 0.0f : top_run) - kWeightTop, c0 = m0.y - base, c1 = m1.y - base;
+          tmem_ld_wait();
+          if (CAP) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * drop);
-              tmem_st_16(o_at + 16 * i, o);
+            for (int e = 0; e < 32; ++e)
+              v[e] = __float_as_uint(fmaf(soft_cap(__uint_as_float(v[e]) * (e < 16 ? f0 : f1), a.cap, inv_cap), kLog2e, e < 16 ? c0 : c1));
+          } else {
+            const uint64_t f[2] = {pack2(f0, f0), pack2(f1, f1)}, c[2] = {pack2(c0, c0), pack2(c1, c1)};
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float p0, p1;
+              unpack2(fma2(pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f[e >> 4], c[e >> 4]), p0, p1);
+              v[e] = __float_as_uint(p0);
+              v[e + 1] = __float_as_uint(p1);
             }
-            tmem_st_wait();
           }
-          drop = 1.0f;
+          if (SLOPES) {
+            const float from = pos - (float)(key + 32 * i);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fmaf(-slope, fabsf(from - (float)e), __uint_as_float(v[e])));
+          }
+          if (edge) {
+            const int n = limit - key - 32 * i, n0 = m0.w == 0.0f ? 0 : n, n1 = m1.w == 0.0f ? 0 : n;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (e >= (e < 16 ? n0 : n1)) v[e] = 0xFF800000u;
+          }
+          float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) high[e >> 1 & 3] = max3(high[e >> 1 & 3], __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+          return fmaxf(max3(high[0], high[1], high[2]), high[3]);
+        };
+        // O may change once the product of the step before is complete, and every phase of its barrier is waited for in turn.
+        auto settle = [&]() {
+          if (j > 0) ok = wait_warp(bar(PV, slot), (j - 1) & 1u, abort_flag, (1u << 24) | (2u << 16) | (j & 0xFFFF));
+          tc_fence_after();
+          if (ok && __any_sync(0xFFFFFFFFu, drop != 1.0f)) {
+            if (j > 0 || !fresh) {
+#pragma unroll 1
+              for (int i = 0; i < D / 16; ++i) {
+                uint32_t o[16];
+                tmem_ld_16c(o_at + 16 * i, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * drop);
+                tmem_st_16(o_at + 16 * i, o);
+              }
+              tmem_st_wait();
+            }
+            drop = 1.0f;
+          }
+        };
+        // A row without a maximum yet gets that of these scores.
+        if (__any_sync(0xFFFFFFFFu, top_run == -INFINITY)) {
+          float first = -INFINITY;
+          const bool none = top_run == -INFINITY;
+#pragma unroll 1
+          for (int i = 0; i < BN / 32; ++i) {
+            uint32_t v[32];
+            first = fmaxf(first, exponents(i, v));
+          }
+          if (none) top_run = first - kWeightTop;
         }
-      };
-      // A row without a maximum yet gets that of these scores.
-      if (__any_sync(0xFFFFFFFFu, top_run == -INFINITY)) {
-        float first = -INFINITY;
-        const bool none = top_run == -INFINITY;
+        // The weights, relative to the maximum of the steps before.
 #pragma unroll 1
         for (int i = 0; i < BN / 32; ++i) {
           uint32_t v[32];
-          first = fmaxf(first, exponents(i, v));
-        }
-        if (none) top_run = first - kWeightTop;
-      }
-      // The weights, relative to the maximum of the steps before.
-#pragma unroll 1
-      for (int i = 0; i < BN / 32; ++i) {
-        uint32_t v[32];
-        float now = exponents(i, v);
-        uint32_t w[16];
-        uint64_t t[2];
-        for (;;) {  // (as a rule once; the exponentials do not wait for the vote: without slopes 377 us with it ahead, 362 like this)
-          t[0] = t[1] = 0;
+          float now = exponents(i, v);
+          uint32_t w[16];
+          uint64_t t[2];
+          for (;;) {  // (as a rule once; the exponentials do not wait for the vote: without slopes 377 us with it ahead, 362 like this)
+            t[0] = t[1] = 0;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float p0 = ex2_approx_ftz(__uint_as_float(v[e])), p1 = ex2_approx_ftz(__uint_as_float(v[e + 1]));
-            t[e >> 4] = add2(t[e >> 4], pack2(p0, p1));
-            w[e / 2] = pack_half2(p0, p1);
-          }
-          if (__builtin_expect(!__any_sync(0xFFFFFFFFu, now > kWeightTop + kLazy), 1)) break;
-          // more than f16 has: the maximum moves by a whole power of two, and all there is down, the weights of this step that are
-          // stored already too (in fp32: f16 may not have the factor)
-          const float by = now > kWeightTop + kLazy ? ceilf(now - kWeightTop) : 0.0f, f = ex2_approx_ftz(-by);
-          if (by > 0.0f) top_run += by;
-          now -= by;
-          l *= f;
-          drop *= f;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) - by);
-          tmem_st_wait();
-#pragma unroll 1
-          for (int z = 0; z < i; ++z) {
-            uint32_t u[16];
-            tmem_ld_16c(p_at + 16 * z, u);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
-              u[e] = pack_half2(p.x * f, p.y * f);
+            for (int e = 0; e < 32; e += 2) {
+              const float p0 = ex2_approx_ftz(__uint_as_float(v[e])), p1 = ex2_approx_ftz(__uint_as_float(v[e + 1]));
+              t[e >> 4] = add2(t[e >> 4], pack2(p0, p1));
+              w[e / 2] = pack_half2(p0, p1);
             }
-            tmem_st_16(p_at + 16 * z, u);
+            if (__builtin_expect(!__any_sync(0xFFFFFFFFu, now > kWeightTop + kLazy), 1)) break;
+            // more than f16 has: the maximum moves by a whole power of two, and all there is down, the weights of this step that are
+            // stored already too (in fp32: f16 may not have the factor)
+            const float by = now > kWeightTop + kLazy ? ceilf(now - kWeightTop) : 0.0f, f = ex2_approx_ftz(-by);
+            if (by > 0.0f) top_run += by;
+            now -= by;
+            l *= f;
+            drop *= f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) - by);
+            tmem_st_wait();
+#pragma unroll 1
+            for (int z = 0; z < i; ++z) {
+              uint32_t u[16];
+              tmem_ld_16c(p_at + 16 * z, u);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+                u[e] = pack_half2(p.x * f, p.y * f);
+              }
+              tmem_st_16(p_at + 16 * z, u);
+            }
           }
+          float t0, t1;
+          unpack2(t[0], t0, t1);
+          l = fmaf(t0 + t1, m0.z, l);
+          unpack2(t[1], t0, t1);
+          l = fmaf(t0 + t1, m1.z, l);
+          // (over scores that have been read, where the weights have no columns of their own)
+          tmem_st_16(p_at + 16 * i, w);
         }
-        float t0, t1;
-        unpack2(t[0], t0, t1);
-        l = fmaf(t0 + t1, m0.z, l);
-        unpack2(t[1], t0, t1);
-        l = fmaf(t0 + t1, m1.z, l);
-        // (over scores that have been read, where the weights have no columns of their own)
-        tmem_st_16(p_at + 16 * i, w);
+        settle();
+        if (!ok) break;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(PFULL, buf));
       }
-      settle();
-      if (!ok) break;
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(PFULL, buf));
+      if (ok && steps > 0) ok = wait_warp(bar(PV, slot), (steps - 1) & 1u, abort_flag, (1u << 24) | (3u << 16));
+      fresh = band < 0;
+      if (!next_pass()) break;
+      if (fresh) top_run = -INFINITY, l = 0.0f;
     }
-    if (ok && steps > 0) ok = wait_warp(bar(PV, slot), (steps - 1) & 1u, abort_flag, (1u << 24) | (3u << 16));
     tc_fence_after();
     // The output through shared memory (this row tile of q is done with), 2 D bytes of each row at a time: whole rows go to
     // memory, where a row a thread would write half sectors.
@@ -479,12 +515,18 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     };
     int page = raw_page(0), page_next = raw_page(1);
     float ks = 0.0f, vs = 0.0f;
-    bool there = false;
+    bool there = false, fresh = true;  // fresh: no band has been taken yet
+    float lowest = INFINITY, highest = -INFINITY;  // of this lane's units' value scales, to base 2
+    uint32_t seen = 0;                             // their bands
     // Where the units of a step lie, through shared memory to the warp's lanes; -1: no page.
     int64_t* offs = reinterpret_cast<int64_t*>(smem + L::kOff) + (warp - 12) * 2 * GR;
     auto look_up = [&](int step) {
       there = page >= 0 && page < a.pages;
       const int key = key_of(step) + 16 * lane;
+      if (band >= 0 && there) {  // what is not of the band counts as no page (zero scales: of the first one)
+        const float scale = __ldg(a.vs + (int64_t)page * a.H + h);
+        there = scale == 0.0f ? fresh : band_of(log2_approx(scale)) == band;
+      }
       if (lane < GR) offs[(step & 1) * GR + lane] = there ? (((int64_t)page * a.H + h) * a.P + key % a.P) * D : -1;
       ks = there ? __ldg(a.ks + (int64_t)page * a.H + h) : 0.0f;
       vs = there ? __ldg(a.vs + (int64_t)page * a.H + h) : 0.0f;
@@ -523,107 +565,132 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     };
     bool ok = true;
     uint32_t zero_units = 0;
-    for (int j = -1; j < steps; ++j) {  // (-1: loads only)
-      if (j >= 0) {
-      const int s = j & 1;
-      const uint32_t phase = (j >> 1) & 1u;
-      // pages with a value scale of zero: their weights count, their values are zeros
-      const float vs_now = vs;
-      zero_units = __ballot_sync(0xFFFFFFFFu, vs_now == 0.0f);
-      const uint32_t holes = __ballot_sync(0xFFFFFFFFu, lane < GR && !there);
-      if (warp == 12 && lane == 0) *reinterpret_cast<int*>(smem + L::kHole + (j & 3) * 4) = holes != 0;
-      if (warp == 12 && lane < GR) {
-        const float lv = vs_now == 0.0f ? kNilLog2 : log2_approx(vs_now);
-        *reinterpret_cast<float4*>(smem + L::kMeta + (j & 3) * GR * 16 + lane * 16) =
-            make_float4(ks, lv, vs_now == 0.0f ? kNilInverse : 1.0f / vs_now, there ? 1.0f : 0.0f);
-      }
-      ok = wait_warp(bar(KEMPTY, s), phase ^ 1u, abort_flag, (2u << 24) | (4u << 16) | (j & 0xFFFF));
-      if (!ok) break;
-      write(k_at + s * L::kTile, kr);
-      if (lane == 0) mbar_arrive(bar(KFULL, s));
-      // (zero_units: of this step, the look-up below is the next one's)
-      }
-      if (j + 1 < steps) {
+    for (;;) {
+      for (int j = -1; j < steps; ++j) {  // (-1: loads only)
         if (j >= 0) {
-          page = page_next;
-          page_next = raw_page(j + 2);
+        const int s = j & 1;
+        const uint32_t phase = (j >> 1) & 1u;
+        // pages with a value scale of zero: their weights count, their values are zeros
+        const float vs_now = vs;
+        zero_units = __ballot_sync(0xFFFFFFFFu, vs_now == 0.0f);
+        const uint32_t holes = __ballot_sync(0xFFFFFFFFu, lane < GR && !there);
+        if (warp == 12 && lane == 0) *reinterpret_cast<int*>(smem + L::kHole + (j & 3) * 4) = holes != 0;
+        if (warp == 12 && lane < GR) {
+          const float lv = vs_now == 0.0f ? kNilLog2 : log2_approx(vs_now);
+          if (vs_now != 0.0f) {
+            lowest = fminf(lowest, lv);
+            highest = fmaxf(highest, lv);
+            seen |= 1u << band_of(lv);
+          }
+          *reinterpret_cast<float4*>(smem + L::kMeta + (j & 3) * GR * 16 + lane * 16) =
+              make_float4(ks, lv, vs_now == 0.0f ? kNilInverse : 1.0f / vs_now, there ? 1.0f : 0.0f);
         }
-        look_up(j + 1);
-        load(a.k, j + 1, kr);
-      }
-      if (j >= 0) {
-      const int s = j & 1;
-      const uint32_t phase = (j >> 1) & 1u;
-      // NaN codes become zeros, and where the first one of a column is goes to the output's warps
+        ok = wait_warp(bar(KEMPTY, s), phase ^ 1u, abort_flag, (2u << 24) | (4u << 16) | (j & 0xFFFF));
+        if (!ok) break;
+        write(k_at + s * L::kTile, kr);
+        if (lane == 0) mbar_arrive(bar(KFULL, s));
+        // (zero_units: of this step, the look-up below is the next one's)
+        }
+        if (j + 1 < steps) {
+          if (j >= 0) {
+            page = page_next;
+            page_next = raw_page(j + 2);
+          }
+          look_up(j + 1);
+          load(a.k, j + 1, kr);
+        }
+        if (j >= 0) {
+        const int s = j & 1;
+        const uint32_t phase = (j >> 1) & 1u;
+        // NaN codes become zeros, and where the first one of a column is goes to the output's warps
 #pragma unroll
-      for (int i = 0; i < UN; ++i) {
-        const int t = i * TPI + first;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&vr[i]);
-        const uint32_t hit = __vcmpeq4(w[0] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) | __vcmpeq4(w[1] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) |
-                             __vcmpeq4(w[2] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) | __vcmpeq4(w[3] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-        if (hit) {
-          *nan_any = 1;
-          vr[i] = without_nans(vr[i], nan_at + chunk * 16, key_of(j) + t);
+        for (int i = 0; i < UN; ++i) {
+          const int t = i * TPI + first;
+          uint32_t* w = reinterpret_cast<uint32_t*>(&vr[i]);
+          const uint32_t hit = __vcmpeq4(w[0] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) | __vcmpeq4(w[1] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) |
+                               __vcmpeq4(w[2] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) | __vcmpeq4(w[3] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+          if (hit) {
+            *nan_any = 1;
+            vr[i] = without_nans(vr[i], nan_at + chunk * 16, key_of(j) + t);
+          }
+          if (zero_units >> (t >> 4) & 1u) w[0] = w[1] = w[2] = w[3] = 0;
         }
-        if (zero_units >> (t >> 4) & 1u) w[0] = w[1] = w[2] = w[3] = 0;
+        ok = wait_warp(bar(VEMPTY, s), phase ^ 1u, abort_flag, (2u << 24) | (5u << 16) | (j & 0xFFFF));
+        if (!ok) break;
+        write(v_at + s * L::kTile, vr);
+        if (lane == 0) mbar_arrive(bar(VFULL, s));
+        }
+        if (j + 1 < steps) load(a.v, j + 1, vr);
       }
-      ok = wait_warp(bar(VEMPTY, s), phase ^ 1u, abort_flag, (2u << 24) | (5u << 16) | (j & 0xFFFF));
-      if (!ok) break;
-      write(v_at + s * L::kTile, vr);
-      if (lane == 0) mbar_arrive(bar(VFULL, s));
+      if (warp == 12 && band < 0) {
+#pragma unroll
+        for (int z = 16; z > 0; z >>= 1) {
+          lowest = fminf(lowest, __shfl_xor_sync(0xFFFFFFFFu, lowest, z));
+          highest = fmaxf(highest, __shfl_xor_sync(0xFFFFFFFFu, highest, z));
+        }
+        seen = __reduce_or_sync(0xFFFFFFFFu, seen);
+        if (lane == 0 && highest - lowest > kFar) *far_bands = seen;
       }
-      if (j + 1 < steps) load(a.v, j + 1, vr);
+      fresh = band < 0;
+      if (!next_pass()) break;
+      page = raw_page(0);
+      page_next = raw_page(1);
     }
     grid_launch_dependents();
-  } else if (warp < 4) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (warp == 0 && elect_one() && steps > 0) {
-      constexpr uint32_t id_s = idesc_f16(128, BN, false), id_o = idesc_f16(128, D, true);
-      auto scores = [&](int j, int slot, int buf) {
-        const uint64_t dq = make_kmajor_sw128_desc(q_at + slot * L::kQ), dk = make_kmajor_sw128_desc(k_at + (j & 1) * L::kTile);
+  } else {
+    // ------------------------------------------------------------------ MMA issuer (warps without a part only keep the passes)
+    bool fresh = true;
+    for (;;) {
+      if (warp == 0 && elect_one() && steps > 0) {
+        constexpr uint32_t id_s = idesc_f16(128, BN, false), id_o = idesc_f16(128, D, true);
+        auto scores = [&](int j, int slot, int buf) {
+          const uint64_t dq = make_kmajor_sw128_desc(q_at + slot * L::kQ), dk = make_kmajor_sw128_desc(k_at + (j & 1) * L::kTile);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_f16_ss(tmem + kS + buf * BN, dq + ((k >> 2) * 128 * 128 + (k & 3) * 32) / 16, dk + ((k >> 2) * BN * 128 + (k & 3) * 32) / 16,
-                     id_s, k > 0);
-        mma_commit(bar(SFULL, buf));
-      };
-      auto product = [&](int j, int slot, int buf) {
-        const uint64_t dv = make_mnmajor_desc(v_at + (j & 1) * L::kTile, BN * 128);
+          for (int k = 0; k < D / 16; ++k)
+            mma_f16_ss(tmem + kS + buf * BN, dq + ((k >> 2) * 128 * 128 + (k & 3) * 32) / 16, dk + ((k >> 2) * BN * 128 + (k & 3) * 32) / 16,
+                       id_s, k > 0);
+          mma_commit(bar(SFULL, buf));
+        };
+        auto product = [&](int j, int slot, int buf) {
+          const uint64_t dv = make_mnmajor_desc(v_at + (j & 1) * L::kTile, BN * 128);
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          mma_f16_ts(tmem + kO + slot * D, tmem + L::kP + buf * L::kPStride + 8 * k, dv + k * 2048 / 16, id_o, j > 0 || k > 0);
-        mma_commit(bar(PV, slot));
-      };
-      // Scores are AHEAD steps ahead of products: one with two row tiles in turn, two with two buffers.
-      constexpr int AHEAD = NQ == 2 ? 1 : 2;
-      bool ok = wait_one(bar(QFULL, 0), 0, abort_flag, (3u << 24) | (6u << 16));
+          for (int k = 0; k < BN / 16; ++k)
+            mma_f16_ts(tmem + kO + slot * D, tmem + L::kP + buf * L::kPStride + 8 * k, dv + k * 2048 / 16, id_o, j > 0 || k > 0 || !fresh);
+          mma_commit(bar(PV, slot));
+        };
+        // Scores are AHEAD steps ahead of products: one with two row tiles in turn, two with two buffers.
+        constexpr int AHEAD = NQ == 2 ? 1 : 2;
+        bool ok = wait_one(bar(QFULL, 0), 0, abort_flag, (3u << 24) | (6u << 16));  // (of the first pass)
 #pragma unroll 1
-      for (int j = -AHEAD; ok && j < steps; ++j) {
-        const int n = j + AHEAD;  // whose scores are next
+        for (int j = -AHEAD; ok && j < steps; ++j) {
+          const int n = j + AHEAD;  // whose scores are next
 #pragma unroll 1
-        for (int slot = 0; ok && slot < NQ; ++slot) {
-          const int buf = NQ == 2 ? slot : j & 1;
-          if (j >= 0) {
-            if (slot == 0) ok = wait_one(bar(VFULL, j & 1), (j >> 1) & 1u, abort_flag, (3u << 24) | (8u << 16) | (j & 0xFFFF));
-            ok = ok && wait_one(bar(PFULL, buf), NQ == 2 ? j & 1u : (j >> 1) & 1u, abort_flag, (3u << 24) | (9u << 16) | (j & 0xFFFF));
-            if (!ok) break;
-            tc_fence_after();
-            product(j, slot, buf);
+          for (int slot = 0; ok && slot < NQ; ++slot) {
+            const int buf = NQ == 2 ? slot : j & 1;
+            if (j >= 0) {
+              if (slot == 0) ok = wait_one(bar(VFULL, j & 1), (j >> 1) & 1u, abort_flag, (3u << 24) | (8u << 16) | (j & 0xFFFF));
+              ok = ok && wait_one(bar(PFULL, buf), NQ == 2 ? j & 1u : (j >> 1) & 1u, abort_flag, (3u << 24) | (9u << 16) | (j & 0xFFFF));
+              if (!ok) break;
+              tc_fence_after();
+              product(j, slot, buf);
+            }
+            if (n < steps) {
+              if (slot == 0) ok = wait_one(bar(KFULL, n & 1), (n >> 1) & 1u, abort_flag, (3u << 24) | (7u << 16) | (n & 0xFFFF));
+              if (L::kOver && j >= 0) ok = ok && wait_one(bar(PV, slot), j & 1u, abort_flag, (3u << 24) | (10u << 16) | (j & 0xFFFF));
+              if (!ok) break;
+              tc_fence_after();
+              scores(n, slot, buf);
+            }
           }
-          if (n < steps) {
-            if (slot == 0) ok = wait_one(bar(KFULL, n & 1), (n >> 1) & 1u, abort_flag, (3u << 24) | (7u << 16) | (n & 0xFFFF));
-            if (L::kOver && j >= 0) ok = ok && wait_one(bar(PV, slot), j & 1u, abort_flag, (3u << 24) | (10u << 16) | (j & 0xFFFF));
-            if (!ok) break;
-            tc_fence_after();
-            scores(n, slot, buf);
-          }
+          // given back only where a later step waits for it
+          if (ok && j >= 0 && j + 2 < steps) mma_commit(bar(VEMPTY, j & 1));
+          if (ok && n + 2 < steps) mma_commit(bar(KEMPTY, n & 1));
         }
-        // given back only where a later step waits for it
-        if (ok && j >= 0 && j + 2 < steps) mma_commit(bar(VEMPTY, j & 1));
-        if (ok && n + 2 < steps) mma_commit(bar(KEMPTY, n & 1));
       }
+      __syncwarp();
+      fresh = band < 0;
+      if (!next_pass()) break;
     }
-    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();

@@ -131,8 +131,12 @@ def cache_attention(q: torch.Tensor, cache: KVCache8, table: torch.Tensor, lens:
     ``q_lens`` [B] int32: only the first ``q_lens[b]`` tokens of a row are there; the rows of ``out`` behind them are left
     as they were.  A query that sees no key gets zeros.  A length above what the table holds counts as what it holds;
     tokens of a page that is no page of the cache are masked.  Keys and values that a query does not see may hold
-    anything.  A value scale is 0 (the page's values are zeros) or lies between 2^-60 and 2^60.  ``out`` must not overlap
-    itself, nor ``q`` unless it is ``q``.  A table holds 2^30 tokens of a sequence at most, a call B up to 65535 and T * heads_q
+    anything.  A value scale is 0 (the page's values are zeros) or lies between 2^-60 and 2^60, those of a sequence's pages within
+    2^96 of one another (more than 2^6 costs time: many rows take a pass for each 2^6 that has pages).  ``out`` must not overlap
+    itself, nor ``q`` unless it is ``q``.
+
+    Scores and all sums are float32.  The weights enter the product as float16: 2^-11 off each, or 2^-29 of the row's largest
+    probability where that is more.  A table holds 2^30 tokens of a sequence at most, a call B up to 65535 and T * heads_q
     up to eight million.
 
     ``workspace``: see ``attention_workspace``; without one a sequence is not shared among multiprocessors."""

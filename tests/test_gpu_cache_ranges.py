@@ -109,3 +109,55 @@ def test_a_long_tail_of_small_weights(D, depth, place, dtype):
     lift = torch.full((n // 64, 1), 2.0 ** 6, device=DEV)
     cache, table = cache_of(k, v, torch.ones_like(lift), lift, 64)
     check(rows_of(D, dtype=dtype), cache, table, n, math.log(2.0), FLUSH)
+
+
+# Value scales within 2^6 of one another share the running maximum (2^-35 of it is then 2^-29 of the row's largest probability, in units
+# of the page's own values), others have one of their own; twice that as above.
+FAR = 2.0 ** -28
+
+
+def scaled_cache(D, page, scales, seed, heads=1, depth=0.0):
+    """Pages with the given value scales (to base 2; None: zero), each with values in every sixteenth column only, so that a column has
+    nothing but its own pages'.  The page with the largest scale has a key 2^depth above the rest."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    pages = len(scales)
+    n = pages * page
+    k, v = torch.zeros(n, heads, D, device=DEV), torch.zeros(n, heads, D, device=DEV)
+    k[:, :, 1] = torch.randint(-12, 1, (n, heads), device=DEV, generator=g) / 8.0
+    for i in range(pages):
+        own = torch.arange(i % 16, D, 16, device=DEV)
+        v[i * page:(i + 1) * page, :, own] = torch.rand(page, heads, own.numel(), device=DEV, generator=g) * 400.0 + 40.0
+    vs = torch.tensor([0.0 if s is None else 2.0 ** s for s in scales], device=DEV)[:, None].expand(pages, heads)
+    k[int(vs[:, 0].argmax()) * page + 3, :, 0] = depth
+    return cache_of(k, v, torch.ones(pages, heads, device=DEV), vs, page, torch.randperm(pages, device=DEV, generator=g)), n
+
+
+@pytest.mark.parametrize("gap", [5, 8, 15, 20, 26, 40, 60, 96])
+@pytest.mark.parametrize("large_first", [False, True])
+@pytest.mark.parametrize("T,D,page", [(1, 64, 16), (1, 128, 64), (2, 256, 32), (90, 128, 16), (90, 256, 128), (90, 64, 256)])
+def test_pages_with_value_scales_far_apart(T, D, page, large_first, gap):
+    """A page with a large scale leaves the others their values, in the columns where it has none."""
+    half = [-gap / 2] * (640 // page) + [gap / 2] * (640 // page)
+    (cache, table), n = scaled_cache(D, page, half[::-1] if large_first else half, gap)
+    check(rows_of(D, T), cache, table, n, math.log(2.0), FAR)
+    (cache, table), n = scaled_cache(D, page, (half * 3)[::-1] if large_first else half * 3, gap, depth=16.0)
+    check(rows_of(D, T), cache, table, n, math.log(2.0), FAR)
+
+
+@pytest.mark.parametrize("T,D,page", [(1, 64, 16), (3, 128, 32), (1, 256, 16), (70, 128, 16), (70, 64, 48), (70, 256, 16)])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+def test_value_scales_over_their_whole_range(T, D, page, order):
+    scales = [-48 + 3 * i for i in range(33)] + [None] * 3
+    if order == "falling":
+        scales.reverse()
+    if order == "mixed":
+        scales = [scales[i * 11 % 36] if i % 2 else scales[-1 - i] for i in range(36)]
+    (cache, table), n = scaled_cache(D, page, scales, 3, heads=2, depth=4.0)
+    check(rows_of(D, T, 8), cache, table, n, math.log(2.0), FAR)
+    check(rows_of(D, T, 8), cache, table, n - page // 2, math.log(2.0), FAR, slopes=torch.full((8,), 2.0 ** -9, device=DEV))
+
+
+def test_value_scales_far_apart_in_f16():
+    for T in (1, 80):
+        (cache, table), n = scaled_cache(128, 16, [0, -9, 3, -8, 0, -6, -9, None] * 6, 5, depth=8.0)
+        check(rows_of(128, T, dtype=torch.float16), cache, table, n, math.log(2.0), FAR)
