@@ -61,8 +61,8 @@ __device__ __forceinline__ void put4(T* p, float a, float b, float c, float d, i
 //
 // Keys on the MMA's M side, 8 rows on its N side.  Every warp walks key tiles of its own with a softmax state of its
 // own, loads (cp.async, one tile ahead, 16-byte pieces swizzled for ldmatrix) and all: no barrier until the end.
-// Codes become f16 in registers, which is exact; q is f16 too, its row brought near 1 by a power of two (a bf16 row keeps
-// all its bits down to 2^-14 of its largest element); weights are f16 with the row's running maximum at 2^10 (kWeightTop).  All sums
+// Codes become f16 in registers, which is exact; q is f16 too, its row brought by a power of two to where f16 ends (a bf16 element
+// keeps all its bits down to 2^-32 of the row's largest, 2^-17 with that at 1; an f16 row loses nothing); weights are f16 with the row's running maximum at 2^10 (kWeightTop).  All sums
 // and the softmax state are fp32.
 //
 // The scales of a page are uniform over 16 keys: ks is part of the scores' factor, vs part of the exponent, as in
@@ -216,9 +216,9 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
     }
     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-    // 2^-e of the largest finite element's exponent e, within what has a normal reciprocal
-    const int e2 = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
-    const float down = __uint_as_float((uint32_t)(254 - e2) << 23), up = __uint_as_float((uint32_t)e2 << 23);
+    // the largest finite element to 2^15 .. 2^16, within what has a normal reciprocal
+    const int e2 = max((int)(__float_as_uint(top) >> 23), 16);
+    const float down = __uint_as_float((uint32_t)(269 - e2) << 23), up = __uint_as_float((uint32_t)(e2 - 15) << 23);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       qf[n][i][0] = pack_half2(value(x[i].x, 0) * down, value(x[i].x, 1) * down);

@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   };
 
   if (warp >= 4 && warp < 12) {
-    // The rows of q as f16, each row's largest element near 1: eight warps, LR lanes a row, eight loads in flight.
+    // The rows of q as f16, each row's largest element near 2^15: eight warps, LR lanes a row, eight loads in flight.
     constexpr int LR = D / 8, RI = 32 / LR, RW = L::ROWS / 8;
     const int piece = lane % LR, from = (warp - 4) * RW;
 #pragma unroll 1
@@ -267,10 +267,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
 #pragma unroll
           for (int z = 1; z < LR; z <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, z));
         }
-        const int e2 = min(max((int)(__float_as_uint(top) >> 23), 2), 252);
-        const float down = __uint_as_float((uint32_t)(254 - e2) << 23);
+        const int e2 = max((int)(__float_as_uint(top) >> 23), 16);  // (as in cache_attn.cu)
+        const float down = __uint_as_float((uint32_t)(269 - e2) << 23);
         const int rr = from + i0 + i * RI + lane / LR, r128 = rr & 127;
-        if (piece == 0) row_factor[rr] = __uint_as_float((uint32_t)e2 << 23) * a.scale;
+        if (piece == 0) row_factor[rr] = __uint_as_float((uint32_t)(e2 - 15) << 23) * a.scale;
         sts128(q_at + (rr >> 7) * L::kQ + (piece >> 3) * 128 * 128 + r128 * 128 + (((piece & 7) ^ (r128 & 7)) << 4),
                pack_half2(v[0] * down, v[1] * down), pack_half2(v[2] * down, v[3] * down), pack_half2(v[4] * down, v[5] * down),
                pack_half2(v[6] * down, v[7] * down));

@@ -136,8 +136,8 @@ def cache_attention(q: torch.Tensor, cache: KVCache8, table: torch.Tensor, lens:
     itself, nor ``q`` unless it is ``q``.
 
     Scores and all sums are float32.  The weights enter the product as float16: 2^-11 off each, or 2^-29 of the row's largest
-    probability where that is more.  A table holds 2^30 tokens of a sequence at most, a call B up to 65535 and T * heads_q
-    up to eight million.
+    probability where that is more; an element of a bfloat16 ``q`` is off by 2^-40 of its row's largest at most.  A table holds
+    2^30 tokens of a sequence at most, a call B up to 65535 and T * heads_q up to eight million.
 
     ``workspace``: see ``attention_workspace``; without one a sequence is not shared among multiprocessors."""
     if native.cache_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, lens, out, causal, prefix, softcap,

@@ -47,6 +47,8 @@ def plain(q, cache, table, n, scale, flush, causal=True, slopes=None, first=0):
         x = q[0, :, i].double()
         s, mag = x @ key.t() * scale, x.abs() @ key.abs().t() * abs(scale)
         err = mag * (D + 8) * 2.0 ** -24
+        if q.dtype == torch.bfloat16:   # q as f16, its largest element at 2^15 or above: half a step of f16's subnormals is 2^-25, so each
+            err = err + 2.0 ** -40 * x.abs().amax(1, keepdim=True) * key.abs().sum(1) * abs(scale)   # element is off by 2^-40 of it at most
         if slopes is not None:
             bias = slopes[i].double() * (p[:, None] - j).abs()
             s, err = s - bias, err + bias * 2.0 ** -22
@@ -161,3 +163,22 @@ def test_value_scales_far_apart_in_f16():
     for T in (1, 80):
         (cache, table), n = scaled_cache(128, 16, [0, -9, 3, -8, 0, -6, -9, None] * 6, 5, depth=8.0)
         check(rows_of(128, T, dtype=torch.float16), cache, table, n, math.log(2.0), FAR)
+
+
+@pytest.mark.parametrize("T,D", [(1, 64), (1, 128), (1, 256), (70, 128), (70, 256)])
+@pytest.mark.parametrize("ratio", [10, 18, 24, 30])
+def test_a_large_element_of_q_where_keys_have_none(T, D, ratio):
+    """The other elements decide the scores: they keep their bits beside it."""
+    g = torch.Generator(device=DEV).manual_seed(ratio)
+    n = 640
+    k, v = (torch.randn(n, 2, D, device=DEV, generator=g) * 60.0 for _ in range(2))
+    k[..., 5] = 0.0
+    for dtype in (torch.bfloat16, torch.float16):
+        if dtype == torch.float16 and ratio > 24:
+            continue
+        low = 1.0 if dtype == torch.bfloat16 else 2.0 ** (14 - ratio)
+        q = (torch.randn(1, T, 8, D, device=DEV, generator=g) * low).to(dtype)
+        q[..., 5] = low * 2.0 ** ratio
+        one = torch.ones(n // 16, 2, device=DEV)
+        cache, table = cache_of(k, v, one / 60.0, one / 60.0, 16)
+        check(q, cache, table, n, 3.0 * D ** -0.5 / low, FAR)
