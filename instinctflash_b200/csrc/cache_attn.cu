@@ -181,8 +181,8 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
   for (int s = 0; s < kStages - 1; ++s) fetch(s, s);
 
   // this thread's columns of the scores: rows 8 n + 2 c + e
-  float factor[NT][2], slope[NT][2], pos[NT][2];
-  int limit[NT][2];
+  float factor[NT][2], slope[NT][2];
+  int limit[NT][2], pos[NT][2];  // pos: the row's position, less the thread's first key in a tile
   uint32_t qf[NT][CH][2];  // q fragments: row 8 n + g, elements 16 i + 4 c .. + 3
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
       factor[n][e] = __shfl_sync(0xFFFFFFFFu, up, (2 * c + e) * 4) * a.scale * (CAP ? 1.0f : kLog2e);
       const int rr = 8 * n + 2 * c + e, tt = (row0 + rr) / a.G;
       limit[n][e] = rr < rows ? limit_of(row0 + rr) : 0;
-      pos[n][e] = (float)(len - nq + tt);
+      pos[n][e] = len - nq + tt - g;
       slope[n][e] = a.slopes && rr < rows ? a.slopes[h * a.G + row0 + rr - tt * a.G] * kLog2e : 0.0f;
     }
   }
@@ -293,11 +293,12 @@ __global__ void __launch_bounds__(32 * kWarps) cache_attend_rows_kernel(const __
         }
       }
       if (a.slopes) {
+        // (whole numbers first: beyond 2^24 positions are no floats)
+        const float from[2] = {(float)(pos[n][0] - key), (float)(pos[n][1] - key)};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            sc[u][n][e] = fmaf(-slope[n][e & 1], fabsf(pos[n][e & 1] - (float)(key + 16 * u + g + (e >> 1) * 8)), sc[u][n][e]);
+          for (int e = 0; e < 4; ++e) sc[u][n][e] = fmaf(-slope[n][e & 1], fabsf(from[e & 1] - (float)(16 * u + (e >> 1) * 8)), sc[u][n][e]);
       }
       if (edge) {
 #pragma unroll

@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
     const int tok = (row0 + (in ? r : 0)) / a.G, hq = h * a.G + (row0 + (in ? r : 0)) - tok * a.G;
     const int limit = in ? limit_of(row0 + r) : INT32_MAX;  // (a row that is not there needs no mask)
     const int least = __reduce_min_sync(0xFFFFFFFFu, limit);
-    const float pos = (float)(len - nq + tok);
+    const int pos = len - nq + tok;
     const float slope = SLOPES ? a.slopes[hq] * kLog2e : 0.0f;
     const float inv_cap = CAP ? 1.0f / a.cap : 0.0f;
     const float factor = row_factor[r];
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
             }
           }
           if (SLOPES) {
-            const float from = pos - (float)(key + 32 * i);
+            const float from = (float)(pos - key - 32 * i);  // (whole numbers first: beyond 2^24 positions are no floats)
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fmaf(-slope, fabsf(from - (float)e), __uint_as_float(v[e])));
           }

@@ -182,3 +182,18 @@ def test_a_large_element_of_q_where_keys_have_none(T, D, ratio):
         one = torch.ones(n // 16, 2, device=DEV)
         cache, table = cache_of(k, v, one / 60.0, one / 60.0, 16)
         check(q, cache, table, n, 3.0 * D ** -0.5 / low, FAR)
+
+
+@pytest.mark.parametrize("T", [1, 3, 80])
+def test_distances_of_far_positions(T):
+    """Slopes count whole tokens beyond 2^24, where float32 has every second one only: a sequence of a few pages over and over."""
+    n, D, page = (1 << 24) + 1003, 64, 256
+    g = torch.Generator(device=DEV).manual_seed(T)
+    k, v = (torch.randn(8 * page, 1, D, device=DEV, generator=g) * 60.0 for _ in range(2))
+    one = torch.ones(8, 1, device=DEV)
+    cache, _ = cache_of(k, v, one / 600.0, one / 60.0, page)
+    table = (torch.arange(-(-n // page), device=DEV) % 8).to(torch.int32).view(1, -1)
+    q = torch.randn(1, T, 2, D, device=DEV, generator=g).to(torch.bfloat16)
+    slopes = torch.tensor([1.0, 0.25], device=DEV)
+    # (4000 tokens back a key has less than e^-900)
+    check(q, cache, table, n, 0.125, FAR, workspaces=(16 << 20,), forms=(1, 2), slopes=slopes, first=n - 4096)
