@@ -282,6 +282,8 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const Appe
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
     for (int w = 0; w < (int)blockDim.x / 32; ++w) top = max(top, tops[w]);
+  } else {
+    __syncwarp();  // (every lane has read the old scale before the first one writes the new)
   }
   const float now = fmaxf(old, page_scale(top));
   uint8_t* codes = a.codes[which] + ((int64_t)page * a.heads + h) * P * D;

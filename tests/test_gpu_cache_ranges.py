@@ -197,3 +197,23 @@ def test_distances_of_far_positions(T):
     slopes = torch.tensor([1.0, 0.25], device=DEV)
     # (4000 tokens back a key has less than e^-900)
     check(q, cache, table, n, 0.125, FAR, workspaces=(16 << 20,), forms=(1, 2), slopes=slopes, first=n - 4096)
+
+
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64), (256, 256)])
+def test_one_token_at_a_time_by_a_warp_repeats_itself(D, page):
+    """Steps of one token, whose page's scale grows at every one: the codes of the page follow one old and one new scale."""
+    sizes = torch.exp2(torch.arange(page, device=DEV) % 24 - 12.0)
+    k = torch.randn(64, page, 2, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(0)) * sizes[:, None, None]
+    table = torch.arange(64, device=DEV, dtype=torch.int32).view(64, 1)
+    caches = [kv_cache.KVCache8.empty(64, 2, page, D, DEV) for _ in range(3)]
+    for c in caches:
+        for i in range(page):
+            kv_cache.cache_append(c, k[:, i:i + 1], -k[:, i:i + 1], table, torch.full((64,), i, device=DEV, dtype=torch.int32))
+        assert torch.equal(c.k_scale, c.v_scale) and torch.equal(c.k.view(torch.uint8) & 0x7F, c.v.view(torch.uint8) & 0x7F)
+        assert torch.equal(c.k.view(torch.uint8), caches[0].k.view(torch.uint8))
+    amax = k.abs().amax(dim=(1, 3))
+    assert ((amax / caches[0].k_scale <= 448.0) & (amax / caches[0].k_scale > 224.0)).all()
+    # every code within half a step of the largest scale's for each time that it moved: it moves exactly, or below the subnormals
+    back = caches[0].k.float() * caches[0].k_scale[:, :, None, None]
+    off = (back - k.transpose(1, 2)).abs()
+    assert (off <= k.transpose(1, 2).abs() * 2.0 ** -4 + caches[0].k_scale[:, :, None, None] * 2.0 ** -10 * 2).all()
