@@ -7,6 +7,8 @@
 // max(position + 1, prefix).
 #include "cache_attn.cuh"
 
+#include <float.h>
+
 namespace iflb200 {
 
 namespace {
@@ -676,7 +678,8 @@ extern "C" int iflb200_cache_attention(const void* q, int dtype, int64_t q_b, in
   if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || page_tokens < 16 || page_tokens > 256 || page_tokens % 16 ||
       heads_q % heads_kv || B > 65535)
     return IFLB200_ERR_SHAPE;
-  if (!(softcap >= 0.0f) || !(scale == scale) || (prefix && !causal)) return IFLB200_ERR_ARG;
+  // (a cap needs a reciprocal, and infinity times tanh(0) is none)
+  if (!(softcap == 0.0f || (softcap >= FLT_MIN && softcap <= FLT_MAX)) || !(fabsf(scale) <= FLT_MAX) || (prefix && !causal)) return IFLB200_ERR_ARG;
   if (B == 0 || T == 0) return IFLB200_OK;
   if (!q || !out || !lens) return IFLB200_ERR_ARG;
   if (pages > 0 && max_pages > 0 && (!k_codes || !v_codes || !k_scale || !v_scale || !table)) return IFLB200_ERR_ARG;

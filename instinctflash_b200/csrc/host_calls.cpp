@@ -25,6 +25,7 @@
 #include <torch/version.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "../../include/iflb200.h"
@@ -837,7 +838,9 @@ PyObject* cache_attention(PyObject*, Args v, Py_ssize_t nargs) {
   const int32_t* q_lens = c.ok ? ints(c, v[13], q.n[0]) : nullptr;
   int64_t bytes = 0;
   void* ws = c.ok ? c.vec(v[14], 0, ScalarType::Byte, &bytes) : nullptr;
-  if (!c.ok || (prefix && !causal) || !(cap >= 0.0) || reinterpret_cast<uintptr_t>(ws) % 16) Py_RETURN_FALSE;
+  if (!c.ok || (prefix && !causal) || !(cap == 0.0 || (cap >= FLT_MIN && cap <= FLT_MAX)) || !(std::fabs(scale) <= FLT_MAX) ||
+      reinterpret_cast<uintptr_t>(ws) % 16)
+    Py_RETURN_FALSE;
   if (v[11] != Py_None && THPVariable_Unpack(v[11]).numel() != q.n[2]) Py_RETURN_FALSE;
   if (!c.ready()) Py_RETURN_FALSE;
   void* s = c.stream();

@@ -158,8 +158,11 @@ def cache_attention(q: torch.Tensor, cache: KVCache8, table: torch.Tensor, lens:
     _ints(prefix, "prefix", (B,), dev)
     if prefix is not None and not causal:
         raise ValueError("prefix goes with causal=True: without it every key is seen")
-    if not softcap >= 0.0:
-        raise ValueError("softcap must be 0 (none) or positive")
+    f32 = torch.finfo(torch.float32)
+    if not (softcap == 0.0 or f32.tiny <= softcap <= f32.max):
+        raise ValueError("softcap must be 0 (none) or a positive, finite, normal float32 number")
+    if scale is not None and not abs(scale) <= f32.max:
+        raise ValueError("scale must be a finite float32 number")
     if slopes is not None and (slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads_q,) or not slopes.is_contiguous()):
         raise ValueError(f"slopes must be a contiguous float32 [{heads_q}] tensor")
     if workspace is not None and (workspace.dtype != torch.uint8 or workspace.ndim != 1 or not workspace.is_contiguous()

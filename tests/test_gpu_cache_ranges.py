@@ -217,3 +217,16 @@ def test_one_token_at_a_time_by_a_warp_repeats_itself(D, page):
     back = caches[0].k.float() * caches[0].k_scale[:, :, None, None]
     off = (back - k.transpose(1, 2)).abs()
     assert (off <= k.transpose(1, 2).abs() * 2.0 ** -4 + caches[0].k_scale[:, :, None, None] * 2.0 ** -10 * 2).all()
+
+
+def test_scalars_that_are_no_normal_numbers_are_refused():
+    one = torch.ones(1, 1, device=DEV)
+    cache, table = cache_of(torch.ones(16, 1, 64, device=DEV), torch.ones(16, 1, 64, device=DEV), one, one, 16)
+    q = rows_of(64)
+    for kw in (dict(softcap=math.inf), dict(softcap=1e-39), dict(softcap=1e39), dict(softcap=-1e-39), dict(scale=math.inf), dict(scale=-1e39),
+               dict(scale=math.nan)):
+        with pytest.raises(ValueError):
+            kv_cache.cache_attention(q, cache, table, ints(16), torch.empty_like(q), **kw)
+    for cap in (1.2e-38, 3e38):   # the ends of what is taken: scores of about the cap, and scores as they are
+        out = kv_cache.cache_attention(q, cache, table, ints(16), torch.empty_like(q), softcap=cap, scale=0.01)
+        assert (out == 1.0).all()
