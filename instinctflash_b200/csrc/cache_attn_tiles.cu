@@ -172,9 +172,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   if (split >= chunks) return;
   const int key0 = split * a.chunk, key1 = min(most, key0 + a.chunk);
   const int steps = (key1 - key0 + BN - 1) / BN;
-  // Steps go from the last keys to the first: with slopes the maximum is among the nearest keys, and stays (from the first key on
-  // it moved at every step: 2048 tokens behind 6144, 32 heads, 507 us, 420 like this).
-  auto key_of = [&](int step) { return key0 + (steps - 1 - step) * BN; };
+  // With slopes steps go from the last keys to the first: the maximum is among the nearest keys, and stays (from the first key on it
+  // moved at every step: 2048 tokens behind 6144, 32 heads, 507 us, 420 like this).  Without them from the first keys on: a row that
+  // sees few keys of its first step has its maximum moved within the next one (from the last on 381 us, 367 like this).
+  auto key_of = [&](int step) { return key0 + (SLOPES ? steps - 1 - step : step) * BN; };
 
   auto start_barriers = [&]() {
     for (int i = 0; i < 2; ++i) {
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
         float4 m0, m1;
         // Exponents of 32 columns (two units).  Everything here is a loop over 32 columns that is not unrolled: the parts of this
         // kernel that run at the same time have to fit the instruction cache together.  With 128 columns unrolled an MMA was
-        // issued every 300 clocks (2048 tokens behind 6144, 32 heads: 746 us then; 495 like this).
+        // issued every 300 clocks (2048 tokens behind 6144, 32 heads: 746 us then, 495 rolled up; 383 with the steps since).
         auto exponents = [&](int i, uint32_t (&v)[32]) {
           tmem_ld_32x32b_x32(s_at + 32 * i, v);
           m0 = lds_f4(m_at + 32 * i);
