@@ -174,8 +174,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attend_tiles_kernel(const _
   const int steps = (key1 - key0 + BN - 1) / BN;
   // With slopes steps go from the last keys to the first: the maximum is among the nearest keys, and stays (from the first key on it
   // moved at every step: 2048 tokens behind 6144, 32 heads, 507 us, 420 like this).  Without them from the first keys on: a row that
-  // sees few keys of its first step has its maximum moved within the next one (from the last on 381 us, 367 like this).
-  auto key_of = [&](int step) { return key0 + (SLOPES ? steps - 1 - step : step) * BN; };
+  // sees few keys of its first step has its maximum moved within the next one (from the last on 381 us, 367 like this; 1024 tokens,
+  // 16 heads of 64 over 4096 keys 67.6 and 63.5).  Head dim 256 goes from the last on all the same (four times 256 tokens over 4096
+  // keys: 174 us, 181 from the first on).
+  constexpr bool kBackward = SLOPES || D == 256;
+  auto key_of = [&](int step) { return key0 + (kBackward ? steps - 1 - step : step) * BN; };
 
   auto start_barriers = [&]() {
     for (int i = 0; i < 2; ++i) {
