@@ -386,7 +386,7 @@ IFLB200_API int iflb200_cache_append(const void* k, int64_t k_b, int64_t k_t, in
  *   s_j = scale * q.k_j;  softcap > 0: s_j = softcap * tanh(s_j / softcap);  slopes: s_j -= slopes[i] * |p - j|
  *   out = sum_j softmax(s)_j v_j  over the keys j < lens[b] and, with causal, j <= p or j < prefix[b] (prefix optional)
  * Scores, weights' sum and output are accumulated in fp32, the weights enter the product as f16 (each off by 2^-11 of it at most,
- * or by 2^-29 of its row's largest probability).  Rows that see no key are zeros; rows t >= q_lens[b] are not written.
+ * or by 2^-28 of its row's largest probability).  Rows that see no key are zeros; rows t >= q_lens[b] are not written.
  * workspace (optional, 16-byte aligned): scratch that lets several CTAs share a sequence; its first 4096 bytes have to be zero
  * and are left so.  Calls that may overlap need one each.
  * scale is finite, softcap 0 or a positive, finite, normal number.  Value scales are 0 or lie between 2^-60 and 2^60, a

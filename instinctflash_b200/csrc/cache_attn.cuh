@@ -40,7 +40,7 @@ constexpr float kNilLog2 = -60.0f, kNilInverse = 1152921504606846976.0f;
 // lost).  A page with a large value scale would take these bits from the other pages', which still are all there is in columns where
 // it has zeros.  So units whose scale is more than 2^6 below the largest one so far get weights with a maximum of their own (few
 // rows), or a pass over the keys for each 2^6 of scales, from the lowest up (row tiles): no weight is off by more than 2^-11 of it or
-// 2^-29 of its row's largest probability, whatever the scales.
+// 2^-28 of its row's largest probability, whatever the scales.
 constexpr float kWeightTop = 10.0f;
 constexpr float kLazy = 5.0f;  // base-2 exponent by which a score may pass the running maximum before it moves: to 2^15
 constexpr float kFar = 6.0f;

@@ -99,7 +99,7 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, table: torch
     2^-6).  A page whose first token is written starts afresh.  Values that are not finite become NaN codes and do not
     enter the scale.  ``counts`` [B] int32: only the first ``counts[b]`` tokens of a row are there.  Tokens whose page lies
     beyond the table, or whose entry is no page of the cache, are dropped, and so is a row with a negative start.  A page must
-    belong to one sequence of the call, and what it holds at and above ``start[b] + counts[b]`` is not kept up."""
+    belong to one sequence of the call, in one place of its table, and what it holds at and above ``start[b] + counts[b]`` is not kept up."""
     if native.cache_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, table, start, counts):
         return
     pages, heads, page_tokens, head_dim = _cache(cache)
@@ -135,11 +135,13 @@ def cache_attention(q: torch.Tensor, cache: KVCache8, table: torch.Tensor, lens:
     2^96 of one another (more than 2^6 costs time: many rows take a pass for each 2^6 that has pages).  ``out`` must not overlap
     itself, nor ``q`` unless it is ``q``.
 
-    Scores and all sums are float32.  The weights enter the product as float16: 2^-11 off each, or 2^-29 of the row's largest
-    probability where that is more; an element of a bfloat16 ``q`` is off by 2^-40 of its row's largest at most.  A table holds
-    2^30 tokens of a sequence at most, a call B up to 65535 and T * heads_q up to eight million.
+    Scores and all sums are float32.  The weights enter the product as float16: 2^-11 off each, or 2^-28 of the row's largest
+    probability where that is more; an element of a bfloat16 ``q`` is off by 2^-40 of its row's largest at most (where that is 2^-111
+    at least).  A table holds 2^30 tokens of a sequence at most, a call B up to 65535 and T * heads_q up to eight million.
 
-    ``workspace``: see ``attention_workspace``; without one a sequence is not shared among multiprocessors."""
+    ``workspace``: see ``attention_workspace``; without one a sequence is not shared among multiprocessors.  How far it is shared
+    goes by what the table holds, not by ``lens``: a table no wider than the longest sequence is the fastest (one sequence of 2048
+    tokens, 8 heads of 128: 1.4 times the time in a table 16 times as wide)."""
     if native.cache_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, table, lens, out, causal, prefix, softcap,
                               slopes, scale, q_lens, workspace):
         return out
