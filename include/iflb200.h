@@ -390,7 +390,7 @@ IFLB200_API int iflb200_cache_append(const void* k, int64_t k_b, int64_t k_t, in
  * workspace (optional, 16-byte aligned): scratch that lets several CTAs share a sequence; its first 4096 bytes have to be zero
  * and are left so.  Calls that may overlap need one each.
  * scale is finite, softcap 0 or a positive, finite, normal number.  Value scales are 0 or lie between 2^-60 and 2^60, a
- * sequence's within 2^96 of one another.  max_pages * page_tokens up to 2^30, B up to 65535.
+ * sequence's within 2^96 of one another (0 counts as 2^-60 there).  max_pages * page_tokens up to 2^30, B up to 65535.
  * No reference counterpart (its cache is 16-bit).
  */
 IFLB200_API int iflb200_cache_attention(const void* q, int dtype, int64_t q_b, int64_t q_t, int64_t q_h, const void* k_codes,

@@ -99,7 +99,8 @@ def cache_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, table: torch
     2^-6).  A page whose first token is written starts afresh.  Values that are not finite become NaN codes and do not
     enter the scale.  ``counts`` [B] int32: only the first ``counts[b]`` tokens of a row are there.  Tokens whose page lies
     beyond the table, or whose entry is no page of the cache, are dropped, and so is a row with a negative start.  A page must
-    belong to one sequence of the call, in one place of its table, and what it holds at and above ``start[b] + counts[b]`` is not kept up."""
+    belong to one sequence of the call, in one place of its table, and what it holds at and above ``start[b] + counts[b]`` is not
+    kept up."""
     if native.cache_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, table, start, counts):
         return
     pages, heads, page_tokens, head_dim = _cache(cache)
@@ -132,8 +133,8 @@ def cache_attention(q: torch.Tensor, cache: KVCache8, table: torch.Tensor, lens:
     as they were.  A query that sees no key gets zeros.  A length above what the table holds counts as what it holds;
     tokens of a page that is no page of the cache are masked.  Keys and values that a query does not see may hold
     anything.  A value scale is 0 (the page's values are zeros) or lies between 2^-60 and 2^60, those of a sequence's pages within
-    2^96 of one another (more than 2^6 costs time: many rows take a pass for each 2^6 that has pages).  ``out`` must not overlap
-    itself, nor ``q`` unless it is ``q``.
+    2^96 of one another, where 0 counts as 2^-60.  More than 2^6 among them costs time: many rows take a pass over the keys for each
+    2^6 that has pages.  ``out`` must not overlap itself, nor ``q`` unless it is ``q``.
 
     Scores and all sums are float32.  The weights enter the product as float16: 2^-11 off each, or 2^-28 of the row's largest
     probability where that is more; an element of a bfloat16 ``q`` is off by 2^-40 of its row's largest at most (where that is 2^-111
